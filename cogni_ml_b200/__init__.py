@@ -6,11 +6,13 @@ library and fails if it has not been built (`python cogni_ml_b200/build.py`).
 """
 from . import synth  # noqa: F401  (numpy only)
 from ._lib import CogniQmmError, lib  # noqa: F401
-from .quant_matmul import (DeviceQuantWeight, GemvMany, QuantMatmul, QuantWeight,  # noqa: F401
-                           TensorType, gemv_many, row_bytes, unpack_top1_keys)
+from .quant_matmul import (ACTIVATIONS, DeviceQuantWeight, GemvMany, QuantMatmul, QuantWeight,  # noqa: F401
+                           TensorType, gemm_glu, gemv_many, row_bytes, unpack_top1_keys)
+from .norm import Norm, norm_residual  # noqa: F401
 from .runner import Projection, QuantProjectionRunner, ResidentSequenceRunner  # noqa: F401
 from .loader import WeightUploader, plan_chunks  # noqa: F401
 
-__all__ = ["CogniQmmError", "DeviceQuantWeight", "GemvMany", "gemv_many", "Projection", "QuantMatmul", "QuantProjectionRunner",
+__all__ = ["ACTIVATIONS", "CogniQmmError", "DeviceQuantWeight", "GemvMany", "gemm_glu", "gemv_many", "Norm",
+           "norm_residual", "Projection", "QuantMatmul", "QuantProjectionRunner",
            "QuantWeight", "ResidentSequenceRunner", "TensorType", "WeightUploader", "lib", "plan_chunks",
            "row_bytes", "synth", "unpack_top1_keys"]

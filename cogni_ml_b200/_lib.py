@@ -43,6 +43,9 @@ SIGNATURES = {
     "cogni_qmm_gemv_top1_noalloc": (_i, [_i, _vp, _vp, _i, _i, _i, C.c_int32, _vp, _vp, _vp, _vp]),
     "cogni_qmm_top1_unpack_keys": (_i, [_vp, _i, _vp, _vp, _vp]),
     "cogni_qmm_gemm_bf16": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "cogni_qmm_gemm_epilogue": (_i, [_vp, _vp]),
+    "cogni_qmm_gemm_glu": (_i, [_vp, _vp]),
+    "cogni_qmm_norm_residual": (_i, [_vp, _vp]),
     "cogni_qmm_matmul_add_host": (_i, [_vp, _i, _i, _vp, _i64, _i, _i, _vp, _vp]),
     "cogni_qmm_release_host_workspaces": (_i, []),
     # include/cogni_qmm_diag.h

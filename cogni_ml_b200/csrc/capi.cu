@@ -6,6 +6,7 @@
 
 #include "host_workspace.cuh"
 #include "qmm_common.cuh"
+#include "row_epilogue.cuh"
 #include "../../include/cogni_qmm_diag.h"
 
 using namespace cogni;
@@ -24,6 +25,49 @@ int check_gemv_args(int type, const void *w, const void *x, const void *y, int i
   if ((reinterpret_cast<uintptr_t>(w) & 15) || (reinterpret_cast<uintptr_t>(x) & 3) ||
       (reinterpret_cast<uintptr_t>(y) & 3))
     return COGNI_QMM_ERR_ALIGN;
+  return COGNI_QMM_OK;
+}
+
+bool aligned_to(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Rows of `width` elements of one of the two output types, `stride` elements apart.
+int check_rows(const void *p, int type, int64_t stride, int width) {
+  if (type != COGNI_QMM_OUT_F32 && type != COGNI_QMM_OUT_BF16) return COGNI_QMM_ERR_ARG;
+  if (stride < width) return COGNI_QMM_ERR_ARG;
+  return aligned_to(p, type == COGNI_QMM_OUT_BF16 ? 2 : 4) ? COGNI_QMM_OK : COGNI_QMM_ERR_ALIGN;
+}
+
+int check_rows_call(const cogni_qmm_gemm_args *a, bool glu, RowsCall &c) {
+  if (!a) return COGNI_QMM_ERR_ARG;
+  if (!supported(a->type)) return COGNI_QMM_ERR_TYPE;
+  if (!a->w || !a->x || !a->y || a->m_rows <= 0 || a->n_out <= 0 || a->k_in <= 0 || a->k_in % 256 != 0)
+    return COGNI_QMM_ERR_ARG;
+  if (a->activation < COGNI_QMM_ACT_NONE || a->activation > COGNI_QMM_ACT_SIGMOID) return COGNI_QMM_ERR_ARG;
+  if ((a->w_up != nullptr) != glu) return COGNI_QMM_ERR_ARG;
+  if (glu && (a->residual || a->y_type != COGNI_QMM_OUT_BF16)) return COGNI_QMM_ERR_ARG;
+  if (!glu && a->bias_up) return COGNI_QMM_ERR_ARG;
+  if (a->m_rows > (1 << 22)) return COGNI_QMM_ERR_LIMIT;
+  if (a->x_stride < a->k_in || a->x_stride % 8 != 0) return COGNI_QMM_ERR_ARG;
+  if (!aligned_to(a->w, 16) || !aligned_to(a->w_up, 16) || !aligned_to(a->x, 16) || !aligned_to(a->bias, 4) ||
+      !aligned_to(a->bias_up, 4))
+    return COGNI_QMM_ERR_ALIGN;
+  int st = check_rows(a->y, a->y_type, a->y_stride, a->n_out);
+  if (!st && a->residual) st = check_rows(a->residual, a->residual_type, a->residual_stride, a->n_out);
+  if (st) return st;
+  c = {};
+  c.type = a->type;
+  c.w = a->w; c.w_up = a->w_up;
+  c.x = a->x; c.x_stride = a->x_stride;
+  c.m_rows = a->m_rows; c.n_out = a->n_out; c.k_in = a->k_in;
+  c.resident = a->resident;
+  RowEpilogue &e = c.epi;
+  e.bias = a->bias; e.bias_up = a->bias_up;
+  e.residual = a->residual; e.residual_stride = a->residual_stride;
+  e.residual_bf16 = a->residual_type == COGNI_QMM_OUT_BF16;
+  e.y = a->y; e.y_stride = a->y_stride; e.y_bf16 = a->y_type == COGNI_QMM_OUT_BF16;
+  e.activation = a->activation;
+  e.vec = rows_vec4(e.y, e.y_stride, e.y_bf16) &&
+          (!e.residual || rows_vec4(e.residual, e.residual_stride, e.residual_bf16));
   return COGNI_QMM_OK;
 }
 
@@ -119,11 +163,15 @@ int cogni_qmm_diag_expire_wait(unsigned limit_us, void *stream) {
   return launch_expire_wait(limit_us, static_cast<cudaStream_t>(stream));
 }
 
-unsigned cogni_qmm_wait_timeouts(void) { return gemv_imma_timeouts() + gemm_prefill_timeouts(); }
+unsigned cogni_qmm_wait_timeouts(void) {
+  return gemv_imma_timeouts() + gemm_prefill_timeouts() + gemm_epilogue_timeouts() + gemm_glu_timeouts();
+}
 
 int cogni_qmm_reset_wait_timeouts(void) {
   int st = gemv_imma_reset_timeouts();
   if (st == COGNI_QMM_OK) st = gemm_prefill_reset_timeouts();
+  if (st == COGNI_QMM_OK) st = gemm_epilogue_reset_timeouts();
+  if (st == COGNI_QMM_OK) st = gemm_glu_reset_timeouts();
   return st;
 }
 
@@ -380,6 +428,38 @@ int cogni_qmm_gemm_bf16(int type, const void *d_w, const void *d_x_bf16, void *d
     return COGNI_QMM_ERR_ALIGN;
   return launch_gemm_prefill(type, d_w, d_x_bf16, d_y, out_type, m_rows, n_out, k_in,
                              static_cast<cudaStream_t>(stream));
+}
+
+int cogni_qmm_gemm_epilogue(const cogni_qmm_gemm_args *args, void *stream) {
+  RowsCall c;
+  const int st = check_rows_call(args, false, c);
+  return st ? st : launch_gemm_epilogue(c, static_cast<cudaStream_t>(stream));
+}
+
+int cogni_qmm_gemm_glu(const cogni_qmm_gemm_args *args, void *stream) {
+  RowsCall c;
+  const int st = check_rows_call(args, true, c);
+  return st ? st : launch_gemm_glu(c, static_cast<cudaStream_t>(stream));
+}
+
+int cogni_qmm_norm_residual(const cogni_qmm_norm_args *a, void *stream) {
+  if (!a || !a->residual || a->m_rows <= 0 || a->n <= 0) return COGNI_QMM_ERR_ARG;
+  if (a->n > 32768) return COGNI_QMM_ERR_LIMIT;
+  if (!a->h && !a->pre.weight) return COGNI_QMM_ERR_ARG;             // nothing to write
+  if ((a->pre.weight != nullptr) != (a->y != nullptr)) return COGNI_QMM_ERR_ARG;
+  if (!a->block && (a->post.weight || a->gate)) return COGNI_QMM_ERR_ARG;
+  for (const cogni_qmm_norm *s : {&a->post, &a->pre}) {
+    if (!s->weight) continue;
+    if (!(s->eps >= 0.f) || (s->kind != COGNI_QMM_NORM_RMS && s->kind != COGNI_QMM_NORM_LAYER)) return COGNI_QMM_ERR_ARG;
+    if (!aligned_to(s->weight, 4) || !aligned_to(s->bias, 4)) return COGNI_QMM_ERR_ALIGN;
+  }
+  int st = check_rows(a->residual, a->residual_type, a->residual_stride, a->n);
+  if (!st && a->block) st = check_rows(a->block, a->block_type, a->block_stride, a->n);
+  if (!st && a->gate) st = check_rows(a->gate, a->gate_type, a->gate_stride ? a->gate_stride : a->n, a->n);
+  if (!st && a->h) st = check_rows(a->h, a->h_type, a->h_stride, a->n);
+  if (!st && a->y) st = check_rows(a->y, a->y_type, a->y_stride, a->n);
+  if (st) return st;
+  return launch_norm_residual(*a, static_cast<cudaStream_t>(stream));
 }
 
 int cogni_qmm_matmul_add_host(const float *x, int rows, int in_dim, const void *w_raw,

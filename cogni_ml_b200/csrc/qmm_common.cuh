@@ -179,6 +179,14 @@ int launch_gemv_top1(int type, const void *d_w, const float *d_x, int in_dim, in
                      long long *d_key, cudaStream_t s);
 int launch_top1_unpack(const long long *d_keys, int batch, int32_t *d_idx, float *d_val,
                        cudaStream_t s);
+struct RowsCall;  // row_epilogue.cuh
+int launch_gemm_epilogue(const RowsCall &c, cudaStream_t s);
+int launch_gemm_glu(const RowsCall &c, cudaStream_t s);
+int launch_norm_residual(const cogni_qmm_norm_args &a, cudaStream_t s);
+unsigned gemm_epilogue_timeouts();
+unsigned gemm_glu_timeouts();
+int gemm_epilogue_reset_timeouts();
+int gemm_glu_reset_timeouts();
 int launch_gemm_prefill(int type, const void *d_w, const void *d_x_bf16, void *d_y, int out_type,
                         int m_rows, int n_out, int k_in, cudaStream_t s);
 

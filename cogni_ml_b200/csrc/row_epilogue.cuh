@@ -1,0 +1,149 @@
+// What happens to a sum of a product with an epilogue on its way to memory: bias, activation, residual
+// or gating, one rounding to the output type.  Shared by the tensor-core prefill kernels
+// (gemm_prefill.cuh) and the kernel for few rows (gemm_rows.cuh).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/cogni_qmm.h"
+
+namespace cogni {
+
+// y[m, n] = residual[m, n] + act(sum + bias[n]), or act(sum_gate + bias[n]) * (sum_up + bias_up[n])
+struct RowEpilogue {
+  const float *bias, *bias_up;  // null: none
+  const void *residual;         // null: none; may be y itself (same strides)
+  void *y;
+  long long residual_stride, y_stride;  // elements between rows
+  int residual_bf16, y_bf16;
+  int activation;
+  int vec;  // four consecutive outputs from a multiple of four on are aligned for one access each
+};
+
+template <int V> struct IntConst { static constexpr int value = V; };
+
+// Calls f with the activation as a constant, so that the choice costs one branch a tile and not one
+// an element.
+template <class F> __device__ __forceinline__ void with_activation(int act, F &&f) {
+  switch (act) {
+    case COGNI_QMM_ACT_RELU: f(IntConst<COGNI_QMM_ACT_RELU>{}); break;
+    case COGNI_QMM_ACT_SILU: f(IntConst<COGNI_QMM_ACT_SILU>{}); break;
+    case COGNI_QMM_ACT_GELU: f(IntConst<COGNI_QMM_ACT_GELU>{}); break;
+    case COGNI_QMM_ACT_GELU_TANH: f(IntConst<COGNI_QMM_ACT_GELU_TANH>{}); break;
+    case COGNI_QMM_ACT_SIGMOID: f(IntConst<COGNI_QMM_ACT_SIGMOID>{}); break;
+    default: f(IntConst<COGNI_QMM_ACT_NONE>{}); break;
+  }
+}
+
+// In f32.  exp(-v) overflows to infinity for v < -88, where v / infinity = -0 and 1 / infinity = 0 are
+// the limits.  The tanh form is v * sigmoid(2 u), the same function without the cancellation of
+// 1 + tanh(u) at negative u.
+template <int ACT> __device__ __forceinline__ float activate(float v) {
+  if (ACT == COGNI_QMM_ACT_RELU) return v < 0.f ? 0.f : v;  // NaN stays NaN
+  if (ACT == COGNI_QMM_ACT_SILU) return __fdividef(v, 1.f + __expf(-v));
+  if (ACT == COGNI_QMM_ACT_SIGMOID) return __fdividef(1.f, 1.f + __expf(-v));
+  if (ACT == COGNI_QMM_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678f));
+  if (ACT == COGNI_QMM_ACT_GELU_TANH)
+    return __fdividef(v, 1.f + __expf(-1.5957691f * (v + 0.044715f * v * v * v)));
+  return v;
+}
+
+__device__ __forceinline__ float bf16_value(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// Plain loads, not through the read-only path: the residual may be the y that other threads write.
+__device__ __forceinline__ float load_residual(const RowEpilogue &e, int m, int n) {
+  if (!e.residual) return 0.f;
+  const long long at = (long long)m * e.residual_stride + n;
+  if (e.residual_bf16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(e.residual)[at]);
+  return reinterpret_cast<const float *>(e.residual)[at];
+}
+__device__ __forceinline__ void store_out(const RowEpilogue &e, int m, int n, float v) {
+  const long long at = (long long)m * e.y_stride + n;
+  if (e.y_bf16) reinterpret_cast<__nv_bfloat16 *>(e.y)[at] = __float2bfloat16_rn(v);
+  else reinterpret_cast<float *>(e.y)[at] = v;
+}
+__device__ __forceinline__ void store_out4(const RowEpilogue &e, int m, int n, const float (&f)[4]) {
+  const long long at = (long long)m * e.y_stride + n;
+  if (e.y_bf16)
+    *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(e.y) + at) =
+        make_uint2(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]));
+  else
+    *reinterpret_cast<float4 *>(reinterpret_cast<float *>(e.y) + at) = make_float4(f[0], f[1], f[2], f[3]);
+}
+// Four outputs n .. n + 3 (n a multiple of four) of row m, those below n_out.
+__device__ __forceinline__ void epilogue_store4(const RowEpilogue &e, const float (&sum)[4], int m, int n, int n_out) {
+  if (n >= n_out) return;
+  const bool vec = e.vec && n + 4 <= n_out;
+  float r[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
+  if (e.residual && vec) {
+    const long long at = (long long)m * e.residual_stride + n;
+    if (e.residual_bf16) {
+      const uint2 b = *reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(e.residual) + at);
+      r[0] = bf16_value(b.x); r[1] = __uint_as_float(b.x & 0xffff0000u);
+      r[2] = bf16_value(b.y); r[3] = __uint_as_float(b.y & 0xffff0000u);
+    } else {
+      const float4 b = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(e.residual) + at);
+      r[0] = b.x; r[1] = b.y; r[2] = b.z; r[3] = b.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = n + i < n_out ? load_residual(e, m, n + i) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) f[i] = sum[i] + (e.bias && n + i < n_out ? __ldg(e.bias + n + i) : 0.f);
+  with_activation(e.activation, [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = r[i] + activate<decltype(act)::value>(f[i]);
+  });
+  if (vec) {
+    store_out4(e, m, n, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (n + i < n_out) store_out(e, m, n + i, f[i]);
+  }
+}
+__device__ __forceinline__ void glu_store4(const RowEpilogue &e, const float (&gate)[4], const float (&up)[4], int m,
+                                           int n, int n_out) {
+  if (n >= n_out) return;
+  float f[4];
+  with_activation(e.activation, [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const bool in = n + i < n_out;
+      f[i] = activate<decltype(act)::value>(gate[i] + (e.bias && in ? __ldg(e.bias + n + i) : 0.f)) *
+             (up[i] + (e.bias_up && in ? __ldg(e.bias_up + n + i) : 0.f));
+    }
+  });
+  if (e.vec && n + 4 <= n_out) {
+    store_out4(e, m, n, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (n + i < n_out) store_out(e, m, n + i, f[i]);
+  }
+}
+
+// Whether four consecutive elements of every row can be one access (rows `stride` elements apart).
+inline bool rows_vec4(const void *p, long long stride, bool bf16) {
+  return (reinterpret_cast<uintptr_t>(p) & (bf16 ? 7 : 15)) == 0 && stride % 4 == 0;
+}
+
+// One call of a product with an epilogue, as the launchers take it.
+struct RowsCall {
+  int type;
+  const void *w, *w_up;  // w_up: gated form
+  const void *x;         // bf16, rows x_stride elements apart
+  long long x_stride;
+  int m_rows, n_out, k_in;
+  int resident;
+  RowEpilogue epi;
+};
+
+}  // namespace cogni

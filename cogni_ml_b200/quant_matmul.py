@@ -17,6 +17,7 @@ fails, without a GPU the calls raise.
 from __future__ import annotations
 
 import enum
+import struct
 import warnings
 from dataclasses import dataclass
 from typing import Optional
@@ -285,6 +286,119 @@ class DeviceQuantWeight:
                                       out.data_ptr(), code, m, self.out_dim, self.in_dim,
                                       _stream_ptr(stream)), "cogni_qmm_gemm_bf16")
         return out
+
+
+    def gemm_epilogue(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+                      residual: Optional[torch.Tensor] = None, out_dtype=torch.float32,
+                      out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """y[m, :] = residual[m, :] + act(W x[m, :] + bias) for any number of rows, x bf16 [M, in_dim].
+
+        activation: one of ACTIVATIONS.  bias f32 [out_dim]; residual [M, out_dim] f32 or bf16, which may
+        be `out` itself.  Rows of x, residual and out may be strided (x by a multiple of eight
+        elements).  A weight enters as bf16(dequant(W)), as in `gemm`."""
+        return _gemm_rows(self, None, x, bias, None, activation, residual, out_dtype, out, stream)
+
+
+#: Names of the activations of `gemm_epilogue` and `gemm_glu`, in the order of COGNI_QMM_ACT_*.
+ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh", "sigmoid")
+_ACT_CODE = {name: code for code, name in enumerate(ACTIVATIONS)}
+_ROW_TYPE = {torch.float32: 0, torch.bfloat16: 1}
+_GEMM_ARGS = struct.Struct("7Q3q8i")  # cogni_qmm_gemm_args
+
+
+def _rows(t: torch.Tensor, width: int, name: str):
+    """(rows, elements between rows) of a tensor whose last dimension has `width` elements."""
+    if t.shape[-1] != width:
+        raise ValueError(f"{name} must have {width} columns, got shape {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t.numel() // width, width
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t.shape[0], t.stride(0) if t.shape[0] > 1 else width
+    raise ValueError(f"{name} must be contiguous, or 2-D with adjacent columns")
+
+
+def _row_type(t: torch.Tensor, name: str) -> int:
+    code = _ROW_TYPE.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be f32 or bf16, got {t.dtype}")
+    return code
+
+
+def _vector(t: Optional[torch.Tensor], n: int, dev: int, name: str) -> int:
+    """Address of an f32 [n] vector on device `dev`, 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name} must be a contiguous f32 tensor of {n} elements on the device of the rows")
+    return t.data_ptr()
+
+
+def _call(fn, what: str, args: bytes, dev: int, stream) -> None:
+    """Launches on device `dev`, whatever device is current."""
+    if dev == torch.cuda.current_device():
+        check(fn(args, _stream_ptr(stream)), what)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(args, _stream_ptr(stream)), what)
+
+
+def _output(rows: int, width: int, like: torch.Tensor, dtype, dev: int, stream) -> torch.Tensor:
+    if dtype not in _ROW_TYPE:
+        raise ValueError(f"outputs are f32 or bf16, not {dtype}")
+    shape = (rows, width) if like.dim() == 2 else like.shape[:-1] + (width,)
+    out = torch.empty(shape, dtype=dtype, device=like.device)
+    if stream:  # allocated on the current stream, written on another
+        out.record_stream(stream)
+    return out
+
+
+def _gemm_rows(w: DeviceQuantWeight, up: Optional[DeviceQuantWeight], x, bias, bias_up, activation, residual,
+               out_dtype, out, stream) -> torch.Tensor:
+    n, k = w.out_dim, w.in_dim
+    dev = x.get_device()
+    if x.dtype != torch.bfloat16 or dev < 0 or w.raw.get_device() != dev:
+        raise ValueError("x must be a bf16 tensor on the device of the weights")
+    act = _ACT_CODE.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {ACTIVATIONS}, got {activation!r}")
+    m, x_stride = _rows(x, k, "x")
+    if up is not None and ((up.type, up.out_dim, up.in_dim) != (w.type, n, k) or up.raw.get_device() != dev):
+        raise ValueError("gate and up must have the same type, shape and device")
+    res_ptr = res_stride = res_type = 0
+    if residual is not None:
+        res_m, res_stride = _rows(residual, n, "residual")
+        if res_m != m or residual.get_device() != dev:
+            raise ValueError("residual must have a row for every row of x, on its device")
+        res_ptr, res_type = residual.data_ptr(), _row_type(residual, "residual")
+    if out is None:
+        out = _output(m, n, x, out_dtype, dev, stream)
+        y_stride = n
+    else:
+        out_m, y_stride = _rows(out, n, "out")
+        if out_m != m or out.get_device() != dev:
+            raise ValueError("out must have a row for every row of x, on its device")
+    y_type = _row_type(out, "out")
+    args = (w.raw.data_ptr(), up.raw.data_ptr() if up is not None else 0, x.data_ptr(), _vector(bias, n, dev, "bias"),
+            _vector(bias_up, n, dev, "bias_up"), res_ptr, out.data_ptr(), x_stride, res_stride, y_stride, w.type, act,
+            res_type, y_type, m, n, k, 1 if w.resident and (up is None or up.resident) else 0)
+    if m == 0:
+        return out
+    if up is None:
+        _call(lib.cogni_qmm_gemm_epilogue, "cogni_qmm_gemm_epilogue", _GEMM_ARGS.pack(*args), dev, stream)
+    else:
+        _call(lib.cogni_qmm_gemm_glu, "cogni_qmm_gemm_glu", _GEMM_ARGS.pack(*args), dev, stream)
+    return out
+
+
+def gemm_glu(gate: DeviceQuantWeight, up: DeviceQuantWeight, x: torch.Tensor, activation: str = "silu",
+             bias_gate: Optional[torch.Tensor] = None, bias_up: Optional[torch.Tensor] = None,
+             out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """y[m, :] = act(Wg x[m, :] + bias_gate) * (Wu x[m, :] + bias_up): the gate and up projections of a
+    feed-forward block and their product in one launch, for any number of rows.  x bf16 [M, in_dim],
+    y bf16 [M, out_dim] (the down projection's input); rows of x and out may be strided."""
+    if out is not None and out.dtype != torch.bfloat16:
+        raise ValueError("out must be bf16")
+    return _gemm_rows(gate, up, x, bias_gate, bias_up, activation, None, torch.bfloat16, out, stream)
 
 
 class GemvMany:

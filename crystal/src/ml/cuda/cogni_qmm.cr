@@ -40,6 +40,66 @@ lib LibCogniQMM
     ticket : UInt32*
   end
 
+  ACT_NONE      = 0
+  ACT_RELU      = 1
+  ACT_SILU      = 2
+  ACT_GELU      = 3
+  ACT_GELU_TANH = 4
+  ACT_SIGMOID   = 5
+  NORM_RMS      = 0
+  NORM_LAYER    = 1
+
+  struct GemmArgs
+    w : DevPtr
+    w_up : DevPtr
+    x : DevPtr
+    bias : DevPtr
+    bias_up : DevPtr
+    residual : DevPtr
+    y : DevPtr
+    x_stride : Int64
+    residual_stride : Int64
+    y_stride : Int64
+    type : Int32
+    activation : Int32
+    residual_type : Int32
+    y_type : Int32
+    m_rows : Int32
+    n_out : Int32
+    k_in : Int32
+    resident : Int32
+  end
+
+  struct Norm
+    weight : DevPtr
+    bias : DevPtr
+    eps : Float32
+    kind : Int32
+  end
+
+  struct NormArgs
+    residual : DevPtr
+    block : DevPtr
+    gate : DevPtr
+    h : DevPtr
+    y : DevPtr
+    residual_stride : Int64
+    block_stride : Int64
+    gate_stride : Int64
+    h_stride : Int64
+    y_stride : Int64
+    post : Norm
+    pre : Norm
+    residual_type : Int32
+    block_type : Int32
+    gate_type : Int32
+    h_type : Int32
+    y_type : Int32
+    scale : Float32
+    m_rows : Int32
+    n : Int32
+  end
+
   fun cogni_qmm_abi_version : Int32
   fun cogni_qmm_status_string(status : Int32) : UInt8*
   fun cogni_qmm_wait_timeouts : UInt32
@@ -102,6 +162,9 @@ lib LibCogniQMM
                                  top_value : DevPtr, stream : Void*) : Int32
   fun cogni_qmm_gemm_bf16(type : Int32, w : DevPtr, x_bf16 : DevPtr, y : DevPtr, out_type : Int32,
                           m_rows : Int32, n_out : Int32, k_in : Int32, stream : Void*) : Int32
+  fun cogni_qmm_gemm_epilogue(args : GemmArgs*, stream : Void*) : Int32
+  fun cogni_qmm_gemm_glu(args : GemmArgs*, stream : Void*) : Int32
+  fun cogni_qmm_norm_residual(args : NormArgs*, stream : Void*) : Int32
   fun cogni_qmm_matmul_add_host(x : Float32*, rows : Int32, in_dim : Int32, w_raw : Void*,
                                 w_bytes : Int64, type : Int32, out_dim : Int32, bias : Float32*,
                                 y : Float32*) : Int32

@@ -51,6 +51,18 @@ extern "C" {
 #define COGNI_QMM_OUT_F32 0
 #define COGNI_QMM_OUT_BF16 1
 
+/* Activations of the products with an epilogue, in f32 on the sum v. */
+#define COGNI_QMM_ACT_NONE 0
+#define COGNI_QMM_ACT_RELU 1
+#define COGNI_QMM_ACT_SILU 2      /* v / (1 + exp(-v))                                        */
+#define COGNI_QMM_ACT_GELU 3      /* v (1 + erf(v / sqrt 2)) / 2                              */
+#define COGNI_QMM_ACT_GELU_TANH 4 /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2        */
+#define COGNI_QMM_ACT_SIGMOID 5   /* 1 / (1 + exp(-v))                                        */
+
+/* Kinds of norm. */
+#define COGNI_QMM_NORM_RMS 0   /* v / sqrt(mean(v^2) + eps) * weight + bias                    */
+#define COGNI_QMM_NORM_LAYER 1 /* (v - mean(v)) / sqrt(var(v) + eps) * weight + bias           */
+
 /* ABI version of the loaded library (== COGNI_QMM_ABI_VERSION it was built with). */
 int cogni_qmm_abi_version(void);
 
@@ -373,6 +385,82 @@ int cogni_qmm_top1_unpack_keys(const int64_t *d_keys, int batch, int32_t *d_top_
  */
 int cogni_qmm_gemm_bf16(int type, const void *d_w, const void *d_x_bf16, void *d_y,
                         int out_type, int m_rows, int n_out, int k_in, void *stream);
+
+/*
+ * The same product with the steps that follow it, for any number of rows: a decode step's single token, the
+ * rows of a serving batch, a chunk of a prompt.  (The reference runs bias, activation, SwiGLU product
+ * and residual addition as kernels of their own, src/ml/cuda/kernels/deltanet_step_probe.ptx:1076, 1324;
+ * src/ml/gguf/qwen35_cpu.cr:1716-1721, src/ml/gguf/nomic_bert.cr for bias and gelu.)
+ *   cogni_qmm_gemm_epilogue  y[m, n] = residual[m, n] + act(sum_k x[m, k] W[n, k] + bias[n])
+ *   cogni_qmm_gemm_glu       y[m, n] = act(sum_k x[m, k] Wg[n, k] + bias[n]) * (sum_k x[m, k] Wu[n, k] + bias_up[n])
+ * The first is an attention output or down projection onto the residual stream, an encoder's biased
+ * matrix, or any projection; the second the gate and up projections of a feed-forward block in one
+ * launch: neither factor is written, y is the bf16 input of the down projection.
+ *
+ *   type      ggml type of the weights (any of the five; gate and up have the same)
+ *   w, w_up   raw GGUF blocks [n_out][k_in], 16-byte aligned; w_up: the up matrix (glu only, w is the gate's;
+ *             cogni_qmm_gemm_epilogue wants it NULL)
+ *   x         bf16 [m_rows, k_in], rows x_stride elements apart (at least k_in, a multiple of 8), 16-byte aligned
+ *   bias, bias_up   NULL, or f32 [n_out]
+ *   residual  NULL, or [m_rows, n_out], f32 or bf16 per residual_type, rows residual_stride (at least n_out)
+ *             apart; it may be y itself (same type and stride).  glu: NULL
+ *   y         [m_rows, n_out], rows y_stride (at least n_out) elements apart, f32 or bf16 per y_type
+ *             (glu: bf16); what lies between the rows is not touched
+ *   k_in a multiple of 256; m_rows at most 4194304
+ *   resident  as in cogni_qmm_gemv_resident, for the weights
+ * Sums, bias, activation and residual are f32, y is rounded once.  cogni_qmm_gemm_epilogue takes a weight
+ * as bf16(dequant(W)), as cogni_qmm_gemm_bf16 does, at any number of rows; cogni_qmm_gemm_glu takes it
+ * so or as the f32 dequant(W), whichever its kernel has.
+ */
+typedef struct cogni_qmm_gemm_args {
+  const void *w, *w_up, *x;
+  const float *bias, *bias_up;
+  const void *residual;
+  void *y;
+  int64_t x_stride, residual_stride, y_stride;
+  int32_t type, activation, residual_type, y_type;
+  int32_t m_rows, n_out, k_in, resident;
+} cogni_qmm_gemm_args;
+
+int cogni_qmm_gemm_epilogue(const cogni_qmm_gemm_args *args, void *stream);
+int cogni_qmm_gemm_glu(const cogni_qmm_gemm_args *args, void *stream);
+
+/*
+ * The norms around a block, with its gate and the addition to the residual stream, in one pass over the
+ * rows:
+ *     h[m, :] = residual[m, :] + scale * gate[m, :] * norm_post(block[m, :])
+ *     y[m, :] = norm_pre(h[m, :])
+ * y is the bf16 input of the products above (or f32), h the residual stream after the block.  (The
+ * reference's rmsnorm / add_rmsnorm kernels, src/ml/cuda/kernels/deltanet_step_probe.ptx:1324;
+ * Qwen35CPU#rms_norm, src/ml/gguf/qwen35_cpu.cr:484-490; the pre and post norms and the layer scale of
+ * src/ml/gguf/gemma4_cpu.cr; the layer norms after the blocks of src/ml/gguf/nomic_bert.cr.)
+ *   residual  [m_rows, n], f32 or bf16 per residual_type
+ *   block     NULL (h = residual), or [m_rows, n]
+ *   post      its norm; post.weight NULL: none.  weight, bias (NULL: none): f32 [n]; eps >= 0
+ *   gate      NULL, or [m_rows, n] factors; gate_stride 0: one row for all
+ *   h         NULL: not written; may be residual itself (same type and stride)
+ *   pre, y    pre.weight NULL: no second norm, y is not written (h is then wanted); y may be block itself
+ *             (same type and stride)
+ * Strides are in elements, at least n; n at most 32768.  Otherwise the outputs overlap no input.  Sums are
+ * f32; h and y are rounded once, y from the f32 h.
+ */
+typedef struct cogni_qmm_norm {
+  const float *weight, *bias;
+  float eps;
+  int32_t kind;
+} cogni_qmm_norm;
+
+typedef struct cogni_qmm_norm_args {
+  const void *residual, *block, *gate;
+  void *h, *y;
+  int64_t residual_stride, block_stride, gate_stride, h_stride, y_stride;
+  cogni_qmm_norm post, pre;
+  int32_t residual_type, block_type, gate_type, h_type, y_type;
+  float scale;
+  int32_t m_rows, n;
+} cogni_qmm_norm_args;
+
+int cogni_qmm_norm_residual(const cogni_qmm_norm_args *args, void *stream);
 
 /*
  * One-shot host-buffer form with the exact call surface of
