@@ -164,7 +164,8 @@ int cogni_qmm_diag_expire_wait(unsigned limit_us, void *stream) {
 }
 
 unsigned cogni_qmm_wait_timeouts(void) {
-  return gemv_imma_timeouts() + gemm_prefill_timeouts() + gemm_epilogue_timeouts() + gemm_glu_timeouts();
+  return gemv_imma_timeouts() + gemm_prefill_timeouts() + gemm_epilogue_timeouts() + gemm_glu_timeouts() +
+         gemm_rows_epilogue_timeouts() + gemm_rows_glu_timeouts();
 }
 
 int cogni_qmm_reset_wait_timeouts(void) {
@@ -172,6 +173,8 @@ int cogni_qmm_reset_wait_timeouts(void) {
   if (st == COGNI_QMM_OK) st = gemm_prefill_reset_timeouts();
   if (st == COGNI_QMM_OK) st = gemm_epilogue_reset_timeouts();
   if (st == COGNI_QMM_OK) st = gemm_glu_reset_timeouts();
+  if (st == COGNI_QMM_OK) st = gemm_rows_epilogue_reset_timeouts();
+  if (st == COGNI_QMM_OK) st = gemm_rows_glu_reset_timeouts();
   return st;
 }
 

@@ -3,7 +3,10 @@
 
 namespace cogni {
 
-int launch_gemm_glu(const RowsCall &c, cudaStream_t s) { return launch_gemm_form<kGlu>(c, s); }
+int launch_gemm_glu(const RowsCall &c, cudaStream_t s) {
+  if (rows_kernel_takes(c)) return launch_gemm_rows_glu(c, s);
+  return launch_gemm_form<kGlu>(c, s);
+}
 
 unsigned gemm_glu_timeouts() { return form_timeouts(); }
 int gemm_glu_reset_timeouts() { return form_reset_timeouts(); }

@@ -39,8 +39,11 @@
 #include <atomic>
 #include <cuda_bf16.h>
 
+#include "cluster_sum.cuh"
+#include "expand.cuh"
 #include "qmm_common.cuh"
 #include "row_epilogue.cuh"
+#include "tensor_map.cuh"
 #include "tma_pipe.cuh"
 
 namespace cogni {
@@ -130,6 +133,7 @@ struct GemmParams {
   long long row_bytes;
   const uint8_t *w_up;  // kGlu: the second matrix (w is the gate's)
   RowEpilogue epi;      // not kPlain: what happens to a sum on its way out
+  float gain;           // kEpilogue: undoes the mean of the accumulation's truncation (mma_gain)
 };
 
 // The tile's A rows.  kGlu: row r is row glu_row(r) of the gate (lanes 0-15 of a quarter) or the up
@@ -221,16 +225,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-// 2-D TMA tile load (no multicast), completion in bytes on an mbarrier.  c0 (the innermost
-// coordinate) times the element size must be a multiple of 16 bytes: here c0 = 64 * k-step.
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *tmap, int c0, int c1,
-                                            uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-      "[%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(tmap), "r"(c0), "r"(c1), "r"(bar)
-      : "memory");
-}
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -246,50 +240,6 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t *>(&v);
-}
-// byte i of v as an exact float
-__device__ __forceinline__ float byte_f(uint32_t v, int i) {
-  return __uint_as_float(__byte_perm(v, 0x4B000000u, 0x7650 + i)) - 8388608.f;
-}
-// byte i of v minus 32 as an exact float: (2^23 + b) - (2^23 + 32)
-__device__ __forceinline__ float byte_f_m32(uint32_t v, int i) {
-  return __uint_as_float(__byte_perm(v, 0x4B000000u, 0x7650 + i)) - 8388640.f;
-}
-// Packed pairs of f32 (sm_100 has two-wide f32 add / mul / fma: same IEEE results per element, half
-// the instructions in the expansion, which is what the dequant warps are bound by).
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint32_t f2_to_bf16x2(uint64_t v) {
-  float a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-  return pack_bf16(a, b);
-}
-// bytes (i, i+1) of v as the floats 2^23 + b, packed
-__device__ __forceinline__ uint64_t bytes2_biased(uint32_t v, int i) {
-  return f2_pack(__uint_as_float(__byte_perm(v, 0x4B000000u, 0x7650 + i)),
-                 __uint_as_float(__byte_perm(v, 0x4B000000u, 0x7650 + i + 1)));
-}
 // Stores chunk c (8 consecutive k elements = 16 bytes) of tile row r at its swizzled position.
 __device__ __forceinline__ void store_chunk(uint8_t *tile, int r, int c, uint4 v) {
   *reinterpret_cast<uint4 *>(tile + r * 128 + ((c ^ (r & 7)) << 4)) = v;
@@ -605,20 +555,13 @@ __device__ __forceinline__ void expand_kstep(const Raw<TYPE> &raw, int ks, int h
   const int j = ks & 3;
   if constexpr (TYPE == kIQ4_NL) {
     // w = d * table[q] (dequant.cr IQ4_NL): element i is the low nibble of byte i, element 16 + i
-    // the high one.  Three byte permutes look four nibbles up (the table's halves by the low three
-    // bits, then a choice by the fourth); two more sort the results into element order.
+    // the high one.  iq4nl_lookup4 looks four nibbles up; two byte permutes sort the results into element order.
     const float d = __half2float(__ushort_as_half((unsigned short)raw.d));
     const uint64_t d_2 = f2_pack(d, d), unbias2 = f2_pack(-8388736.f, -8388736.f);
-    auto lut4 = [](uint32_t hq) {
-      const uint32_t s7 = hq & 0x7777u;
-      const uint32_t lo = __byte_perm(0xBFAD9881u, 0xF6EADDCFu, s7);
-      const uint32_t hi = __byte_perm(0x26190D01u, 0x71594535u, s7);
-      return __byte_perm(lo, hi, 0x3210u | ((hq >> 1) & 0x4444u));
-    };
     uint32_t lows[4], highs[4];  // elements 4i .. 4i+3 and 16+4i .. 16+4i+3 as int8
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const uint32_t a = lut4(raw.q[i]), b = lut4(raw.q[i] >> 16);
+      const uint32_t a = iq4nl_lookup4(raw.q[i]), b = iq4nl_lookup4(raw.q[i] >> 16);
       lows[i] = __byte_perm(a, b, 0x6420);
       highs[i] = __byte_perm(a, b, 0x7531);
     }
@@ -709,37 +652,16 @@ __device__ __forceinline__ void expand_kstep(const Raw<TYPE> &raw, int ks, int h
 // adds up its share of the columns from all of them, in the order of the parts, through distributed
 // shared memory: the same bits launch after launch, nothing to zero, no atomics, and a bf16 y is
 // rounded once like an unsplit one.
-__device__ __forceinline__ uint32_t peer_smem(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ float4 ld_peer4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ void split_sync() {  // all threads of all CTAs of the cluster
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// The sum over the parts of four consecutive tile rows, in the order of the parts.
-__device__ __forceinline__ float4 sum_parts(uint32_t own, int splits) {
-  float4 a = ld_peer4(peer_smem(own, 0));
-  for (int z = 1; z < splits; z++) {
-    const float4 b = ld_peer4(peer_smem(own, z));
-    a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-  }
-  return a;
-}
 // Four outputs n .. n + 3 of token m from their sums (kGlu: g the gate's, u the up's).
 template <int MODE>
 __device__ __forceinline__ void finish4(const GemmParams &p, const float4 &g, const float4 &u, int m, int n) {
   const float gv[4] = {g.x, g.y, g.z, g.w}, uv[4] = {u.x, u.y, u.z, u.w};
-  if (MODE == kGlu) glu_store4(p.epi, gv, uv, m, n, p.n_out);
-  else epilogue_store4(p.epi, gv, m, n, p.n_out);
+  if (MODE == kGlu) {
+    glu_store4(p.epi, gv, uv, m, n, p.n_out);
+  } else {
+    const float v[4] = {p.gain * g.x, p.gain * g.y, p.gain * g.z, p.gain * g.w};
+    epilogue_store4(p.epi, v, m, n, p.n_out);
+  }
 }
 // kEpilogue: brings the residual of columns m .. m + cols, rows n .. n + 31 (one warp's share of a
 // tile) into the L2 while the last MMAs run; read in the epilogue it then costs an L2 hit each 32 tokens.
@@ -797,7 +719,7 @@ __device__ __forceinline__ void store_columns(const GemmParams &p, uint32_t tadd
 #pragma unroll
             for (int j = 0; j < 16; j++)
               if (h + j < live)
-                store_out(p.epi, m0 + c0 + h + j, n, r[j] + activate<decltype(act)::value>(__uint_as_float(v[h + j]) + bias));
+                store_out(p.epi, m0 + c0 + h + j, n, r[j] + activate<decltype(act)::value>(fmaf(p.gain, __uint_as_float(v[h + j]), bias)));
           }
         }
       }
@@ -1409,23 +1331,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 }
 
 // ---------------------------------------------------------------------------- host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
-                                  const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void *ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
-        qres == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  }
-  return fn;
-}
-
 // k-steps of a part of an n-way split: whole superblocks
 int ksteps_per_split(int nks, int splits) { return splits > 1 ? ((nks + splits - 1) / splits + 3) / 4 * 4 : nks; }
 
@@ -1519,6 +1424,14 @@ int encode_maps(const RowsCall &c, int tokens, bool staged, long long row_bytes,
     r = encode_weights<TYPE>(encode, &maps[2], c.w_up, c.n_out, out_rows<MODE>(), row_bytes);
   return (int)r;
 }
+// The tensor core truncates the accumulator at every K = 16 step, which pulls a sum towards zero: by half a unit in
+// the last place of the partial sum, and given its final value y a sum of `steps` terms of any signs stands at
+// y s / steps on average after s of them.  Measured, f32 outputs with K = 2048 .. 32768, weights of four types
+// and activations of mean 0 and 1/2: y comes out (1 - a steps) y, a = 1.30e-8 .. 1.58e-8, about 2^-26.  Taking
+// that mean out halves the error against f64: K = 12288 1.34e-5 -> 6.7e-6 of the norm (a part of a K split
+// counts its own steps).
+float mma_gain(int steps) { return 1.f + (float)steps * 1.4901161e-8f; }
+
 GemmParams gemm_params(const RowsCall &c, long long row_bytes, int splits, int ks_per_split) {
   GemmParams p;
   p.w = static_cast<const uint8_t *>(c.w);
@@ -1530,6 +1443,7 @@ GemmParams gemm_params(const RowsCall &c, long long row_bytes, int splits, int k
   p.splits = splits;
   p.ks_per_split = ks_per_split;
   p.epi = c.epi;
+  p.gain = mma_gain(4 * ks_per_split);
   return p;
 }
 

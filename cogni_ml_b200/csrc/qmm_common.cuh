@@ -182,11 +182,17 @@ int launch_top1_unpack(const long long *d_keys, int batch, int32_t *d_idx, float
 struct RowsCall;  // row_epilogue.cuh
 int launch_gemm_epilogue(const RowsCall &c, cudaStream_t s);
 int launch_gemm_glu(const RowsCall &c, cudaStream_t s);
+int launch_gemm_rows_epilogue(const RowsCall &c, cudaStream_t s);  // gemm_rows.cuh
+int launch_gemm_rows_glu(const RowsCall &c, cudaStream_t s);
 int launch_norm_residual(const cogni_qmm_norm_args &a, cudaStream_t s);
 unsigned gemm_epilogue_timeouts();
 unsigned gemm_glu_timeouts();
 int gemm_epilogue_reset_timeouts();
 int gemm_glu_reset_timeouts();
+unsigned gemm_rows_epilogue_timeouts();
+unsigned gemm_rows_glu_timeouts();
+int gemm_rows_epilogue_reset_timeouts();
+int gemm_rows_glu_reset_timeouts();
 int launch_gemm_prefill(int type, const void *d_w, const void *d_x_bf16, void *d_y, int out_type,
                         int m_rows, int n_out, int k_in, cudaStream_t s);
 

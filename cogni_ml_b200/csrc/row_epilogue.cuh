@@ -146,4 +146,7 @@ struct RowsCall {
   RowEpilogue epi;
 };
 
+// Few rows go to the kernel that streams the weights (gemm_rows.cuh), more to the tensor-core tiles.
+inline bool rows_kernel_takes(const RowsCall &c) { return c.m_rows <= 64; }
+
 }  // namespace cogni
