@@ -74,10 +74,10 @@ __host__ __device__ constexpr int raw_stage_bytes(int type) {
   return type == kQ6_K ? 2 * kRawBox : 128 * (type == kQ5_K ? 176 : 144);  // Q4_K, IQ4_NL: 144
 }
 __host__ __device__ constexpr int raw_bytes(int type, bool staged) { return staged ? 2 * raw_stage_bytes(type) : 0; }
-// stages of the ring that fit beside the raw windows (227 KB per CTA)
-__host__ __device__ constexpr int stages_for(int bn, int raw = 0) {
+// stages of the ring that fit beside the raw windows (227 KB per CTA; 113 KB where two share an SM)
+__host__ __device__ constexpr int stages_for(int bn, int raw = 0, bool two = false) {
   const int want = bn > 256 ? 2 : 4;
-  const int fit = (227 * 1024 - 1024 - 256 - raw) / (128 * 64 * 2 + bn * 64 * 2);
+  const int fit = ((two ? 113 : 227) * 1024 - 1024 - 256 - raw) / (128 * 64 * 2 + bn * 64 * 2);
   return fit < want ? fit : want;
 }
 // Dequant warps: sixteen for Q4_K / Q5_K staged by TMA (four threads per tile row, one per
@@ -86,8 +86,9 @@ __host__ __device__ constexpr int stages_for(int bn, int raw = 0) {
 // against 1216 TFLOP/s, and the same on a CTA pair); eight (two threads
 // per tile row, one per 32-element half of a k-step); four (one thread per row, both halves) for
 // Q6_K read directly from global memory, whose loads are the bound there.
-__host__ __device__ constexpr int dequant_warps(int type, bool staged = false) {
-  if (staged && (type == kQ4_K || type == kQ5_K)) return 16;
+// Two CTAs on an SM (`two`): eight each.
+__host__ __device__ constexpr int dequant_warps(int type, bool staged = false, bool two = false) {
+  if (staged && (type == kQ4_K || type == kQ5_K)) return two ? 8 : 16;
   return type == kQ6_K && !staged ? 4 : 8;
 }
 // Warp roles.  A warp scheduler serves the warps w with the same w % 4, and the thread that issues
@@ -105,8 +106,8 @@ constexpr int kIsoWarps = 22;
 __host__ __device__ constexpr bool isolate_mma_warp(int type, bool staged, int bn) {
   return dequant_warps(type, staged) == 16 && bn == 512;
 }
-__host__ __device__ constexpr int threads_for(int type, bool staged = false, int bn = 512) {
-  return isolate_mma_warp(type, staged, bn) ? 32 * kIsoWarps : 64 + 32 * dequant_warps(type, staged);
+__host__ __device__ constexpr int threads_for(int type, bool staged = false, int bn = 512, bool two = false) {
+  return isolate_mma_warp(type, staged, bn) ? 32 * kIsoWarps : 64 + 32 * dequant_warps(type, staged, two);
 }
 template <bool ISO> struct Roles {
   static constexpr int tma_warp = ISO ? 5 : 0;
@@ -751,15 +752,15 @@ __device__ __forceinline__ void store_columns(const GemmParams &p, uint32_t tadd
 }
 
 // ---------------------------------------------------------------------------- the kernel
-template <int TYPE, int BN, bool STAGED, int MODE>
-__global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN), 1)
+template <int TYPE, int BN, bool STAGED, int MODE, bool TWO>
+__global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 1)
     gemm_prefill_kernel(const __grid_constant__ CUtensorMap tmap_x,
                         const __grid_constant__ CUtensorMap tmap_w,
                         const __grid_constant__ CUtensorMap tmap_up, const GemmParams p) {
   constexpr int kRawStage = raw_stage_bytes(TYPE);
-  constexpr int kStages = stages_for(BN, raw_bytes(TYPE, STAGED));
+  constexpr int kStages = stages_for(BN, raw_bytes(TYPE, STAGED), TWO);
   static_assert(kStages >= 2, "at least two stages");
-  constexpr int kDequantWarps = dequant_warps(TYPE, STAGED);
+  constexpr int kDequantWarps = dequant_warps(TYPE, STAGED, TWO);
   constexpr int kHalves = kDequantWarps >= 8 ? 1 : 2;   // halves of a k-step per thread
   constexpr bool kQuarter = kDequantWarps == 16;        // a thread expands one quarter of a k-step
   constexpr int kBTile = BN * kBK * 2;
@@ -929,7 +930,7 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN), 1)
       // 47.8 -> 44.7, IQ4_NL 44.4 -> 40.6.  Not with sixteen (Q4_K 34.5 -> 35.5), nor where only two
       // or three stages fit and the tensor cores would wait for the pair (256 tokens, Q4_K 38.6 ->
       // 49.8, IQ4_NL 45.7 -> 53.6).
-      constexpr int kBatch = BN == 128 && kDequantWarps == 8 ? 2 : 1;
+      constexpr int kBatch = BN == 128 && kDequantWarps == 8 && !TWO ? 2 : 1;
       for (int ks = 0; ks < nks; ks += kBatch) {  // nks is a multiple of four
         const int sbl = ks >> 2, buf = sbl & 1;
         if ((ks & 3) == 0) mbar_wait(smem_u32(&raw_bars[buf]), (sbl >> 1) & 1);
@@ -1334,17 +1335,17 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // k-steps of a part of an n-way split: whole superblocks
 int ksteps_per_split(int nks, int splits) { return splits > 1 ? ((nks + splits - 1) / splits + 3) / 4 * 4 : nks; }
 
-template <int TYPE, int BN, bool STAGED>
+template <int TYPE, int BN, bool STAGED, bool TWO = false>
 constexpr int smem_for() {
-  return stages_for(BN, raw_bytes(TYPE, STAGED)) * (kATile + BN * kBK * 2) + raw_bytes(TYPE, STAGED) +
+  return stages_for(BN, raw_bytes(TYPE, STAGED), TWO) * (kATile + BN * kBK * 2) + raw_bytes(TYPE, STAGED) +
          1024 /*alignment*/ + 256 /*barriers*/;
 }
-template <int TYPE, int BN, bool STAGED, int MODE>
+template <int TYPE, int BN, bool STAGED, int MODE, bool TWO>
 int configure(int dev) {  // opts into the shared memory, once per device
   static bool configured[64] = {false};
   if (dev < 0 || dev >= 64 || configured[dev]) return COGNI_QMM_OK;
-  cudaError_t e = cudaFuncSetAttribute(gemm_prefill_kernel<TYPE, BN, STAGED, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       smem_for<TYPE, BN, STAGED>());
+  cudaError_t e = cudaFuncSetAttribute(gemm_prefill_kernel<TYPE, BN, STAGED, MODE, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       smem_for<TYPE, BN, STAGED, TWO>());
   if (e != cudaSuccess) return (int)e;
   configured[dev] = true;
   return COGNI_QMM_OK;
@@ -1366,7 +1367,7 @@ void split_launch_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute &attr, dim
 
 // How many clusters of `splits` CTAs run at once (every instance takes a whole SM's shared memory,
 // so the narrowest one stands for all).
-template <int MODE>
+template <int MODE, bool TWO>
 int split_capacity(int dev, int splits) {
   static std::atomic<int> cached[64][9];  // 1 + the count
   if (dev < 0 || dev >= 64) return 0;
@@ -1375,11 +1376,11 @@ int split_capacity(int dev, int splits) {
   if (v == 0) {
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr;
-    split_launch_config(cfg, attr, dim3(1, 1, splits), threads_for(kQ4_K, true, 128), smem_for<kQ4_K, 128, true>(),
+    split_launch_config(cfg, attr, dim3(1, 1, splits), threads_for(kQ4_K, true, 128, TWO), smem_for<kQ4_K, 128, true, TWO>(),
                         splits, nullptr);
     int n = 0;
-    if (configure<kQ4_K, 128, true, MODE>(dev) != COGNI_QMM_OK ||
-        cudaOccupancyMaxActiveClusters(&n, gemm_prefill_kernel<kQ4_K, 128, true, MODE>, &cfg) != cudaSuccess || n < 0) {
+    if (configure<kQ4_K, 128, true, MODE, TWO>(dev) != COGNI_QMM_OK ||
+        cudaOccupancyMaxActiveClusters(&n, gemm_prefill_kernel<kQ4_K, 128, true, MODE, TWO>, &cfg) != cudaSuccess || n < 0) {
       cudaGetLastError();  // no split then
       n = 0;
     }
@@ -1447,7 +1448,7 @@ GemmParams gemm_params(const RowsCall &c, long long row_bytes, int splits, int k
   return p;
 }
 
-template <int TYPE, int BN, bool STAGED, int MODE>
+template <int TYPE, int BN, bool STAGED, int MODE, bool TWO = false>
 int launch(const RowsCall &c, int splits, cudaStream_t s) {
   const long long row_bytes = (long long)(c.k_in / 256) * Sb<TYPE>::bytes;
   CUtensorMap maps[3];
@@ -1455,14 +1456,14 @@ int launch(const RowsCall &c, int splits, cudaStream_t s) {
   if (st) return st;
   int dev = 0;
   cudaGetDevice(&dev);
-  st = configure<TYPE, BN, STAGED, MODE>(dev);
+  st = configure<TYPE, BN, STAGED, MODE, TWO>(dev);
   if (st) return st;
   const GemmParams p = gemm_params(c, row_bytes, splits, ksteps_per_split(c.k_in / kBK, splits));
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr;
   split_launch_config(cfg, attr, dim3((c.n_out + out_rows<MODE>() - 1) / out_rows<MODE>(), (c.m_rows + BN - 1) / BN, splits),
-                      threads_for(TYPE, STAGED, BN), smem_for<TYPE, BN, STAGED>(), splits, s);
-  return (int)cudaLaunchKernelEx(&cfg, gemm_prefill_kernel<TYPE, BN, STAGED, MODE>, maps[0], maps[1], maps[2], p);
+                      threads_for(TYPE, STAGED, BN, TWO), smem_for<TYPE, BN, STAGED, TWO>(), splits, s);
+  return (int)cudaLaunchKernelEx(&cfg, gemm_prefill_kernel<TYPE, BN, STAGED, MODE, TWO>, maps[0], maps[1], maps[2], p);
 }
 
 // The 2-CTA kernel: 256 weight rows x 512 tokens per cluster of two CTAs.
@@ -1549,7 +1550,7 @@ int launch_typed(const RowsCall &c, cudaStream_t s) {
       // Q8_0's direct loads contend where three parts fill the SMs with tiles narrower than the tokens (229 x
       // 2760 x 5376: 128 tokens in three parts 33.7 us, 256 in four on two thirds of the SMs 26.8)
       if (sp == 3 && TYPE == kQ8_0 && widths[i] != 512 && m_rows > widths[i] && g_prefill_force_split != 3) continue;
-      const int at_once = sp == 1 ? sms : split_capacity<MODE>(dev, sp);
+      const int at_once = sp == 1 ? sms : split_capacity<MODE, false>(dev, sp);
       if (at_once == 0) continue;
       const long long tiles = row_tiles * ((m_rows + widths[i] - 1) / widths[i]);
       const int tokens = m_rows < widths[i] ? m_rows : widths[i];
@@ -1558,6 +1559,29 @@ int launch_typed(const RowsCall &c, cudaStream_t s) {
       double cost = (double)((tiles + at_once - 1) / at_once) * t;
       if (g_prefill_force_split >= 2 && sp == g_prefill_force_split) cost -= 1e6;
       if (cost < best) { best = cost; bn = widths[i]; splits = sp; }
+    }
+  }
+  // Tiles of 128 tokens two CTAs an SM, for the forms with an epilogue: a tile's expansion is a chain of latencies, and
+  // two chains of eight warps overlap better than one of sixteen (us: gated Q4_K 12288 x 4096, 128 tokens 66.9 -> 53.4,
+  // Q8_0 8192 x 4096, 100 tokens 38.0 -> 32.4; fitted as above on 33 to 400 tokens, geometric mean over the best plan
+  // 1.06 -> 1.03; tiles of 64 tokens would make it 1.02, and IQ4_NL gains 1.5 %).
+  constexpr bool kTwo = MODE != kPlain && (TYPE == kQ4_K || TYPE == kQ5_K || TYPE == kQ8_0);
+  if constexpr (kTwo) {
+    if ((staged || TYPE == kQ8_0) && !g_prefill_force_bn && g_prefill_force_split == 0) {
+      const double fixed = TYPE == kQ8_0 ? 4.90 : 7.15, step = TYPE == kQ8_0 ? 1.196 : 0.742,
+                   column = TYPE == kQ8_0 ? 0.0029 : 0.0070, lone = TYPE == kQ8_0 ? 0.76 : 0.94;
+      int two_splits = 0;
+      for (int sp : {1, 2, 3, 4, 8}) {
+        const int per = ksteps_per_split(nks, sp);
+        if (sp > 1 && (per < 8 || (sp - 1) * per >= nks)) continue;
+        const int at_once = sp == 1 ? 2 * sms : split_capacity<MODE, true>(dev, sp);
+        if (at_once == 0) continue;
+        const long long tiles = row_tiles * ((m_rows + 127) / 128);
+        const double t = fixed + step * per + (sp > 1 ? column * (m_rows < 128 ? m_rows : 128) : 0.0);
+        const double cost = tiles * sp > sms ? (double)((tiles + at_once - 1) / at_once) * t : lone * t;  // alone on its SM
+        if (cost < best) { best = cost; two_splits = sp; }
+      }
+      if (two_splits) return launch<TYPE, 128, TYPE != kQ8_0, MODE, true>(c, two_splits, s);
     }
   }
   if constexpr (TYPE != kQ8_0) {

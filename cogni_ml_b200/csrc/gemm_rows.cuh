@@ -23,6 +23,8 @@
 // for the preceding kernel (programmatic dependent launch).
 #pragma once
 
+#include <atomic>
+
 #include "cluster_sum.cuh"
 #include "expand.cuh"
 #include "qmm_common.cuh"
@@ -94,13 +96,24 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Four bytes 0 .. 255 to two bf16 pairs: d * (byte - BIAS) or d * byte - m, in f32 as the dequantiser has it
-// (the 2^23 bias comes off exactly), then one rounding.
-template <int BIAS> __device__ __forceinline__ void scale_word(uint32_t q, uint64_t d2, uint32_t &r0, uint32_t &r1) {
-  const uint64_t off = f2_pack(-8388608.f - BIAS, -8388608.f - BIAS);
-  r0 = f2_to_bf16x2(f2_mul(d2, f2_add(bytes2_biased(q, 0), off)));
-  r1 = f2_to_bf16x2(f2_mul(d2, f2_add(bytes2_biased(q, 2), off)));
+// Four bytes to two bf16 pairs, in f32 as the dequantiser has it, then one rounding.  Without a minimum: d (byte - BIAS)
+// as one fma on pairs.  The byte becomes a float by a permute that puts it into the mantissa of a power of
+// two: 128 + byte (Q6_K, byte < 64, BIAS 32) or 2^15 + byte (bytes up to 255, BIAS 128); d has 18 (11) bits, so
+// that power plus BIAS times d (160 = 5 * 2^5, 32896 = 257 * 2^7) is exact in f32 and so is the result.
+template <int BIAS> __device__ __forceinline__ uint64_t scale_offset(float d) {
+  const float c = BIAS == 32 ? -160.f * d : -32896.f * d;
+  return f2_pack(c, c);
 }
+template <int BIAS> __device__ __forceinline__ uint64_t bytes2_float(uint32_t q, int i) {
+  constexpr uint32_t base = BIAS == 32 ? 0x43000000u : 0x47000000u, sel = BIAS == 32 ? 0x7044u : 0x7604u;
+  constexpr int shift = BIAS == 32 ? 8 : 4;
+  return f2_pack(__uint_as_float(__byte_perm(q, base, sel + (i << shift))), __uint_as_float(__byte_perm(q, base, sel + ((i + 1) << shift))));
+}
+template <int BIAS> __device__ __forceinline__ void scale_word(uint32_t q, uint64_t d2, uint64_t c2, uint32_t &r0, uint32_t &r1) {
+  r0 = f2_to_bf16x2(f2_fma(d2, bytes2_float<BIAS>(q, 0), c2));
+  r1 = f2_to_bf16x2(f2_fma(d2, bytes2_float<BIAS>(q, 2), c2));
+}
+// With one: d * byte - m (2^23 + byte, whose bias comes off exactly).
 __device__ __forceinline__ void scale_min_word(uint32_t q, uint64_t d2, uint64_t nm2, uint32_t &r0, uint32_t &r1) {
   const uint64_t off = f2_pack(-8388608.f, -8388608.f);
   r0 = f2_to_bf16x2(f2_fma(d2, f2_add(bytes2_biased(q, 0), off), nm2));
@@ -167,7 +180,7 @@ template <> struct Lane<kQ5_K> : LaneK45<kQ5_K> {};
 // are the half's run b (chunks 0-3), the high ones run 2 + b (chunks 4-7); a run has two scales.
 template <> struct Lane<kQ6_K> {
   uint32_t ql[8], qh[8];
-  uint64_t d[4];  // low run: elements 0-15, 16-31; high run
+  uint64_t d[4], c[4];  // low run: elements 0-15, 16-31; high run
   // eight words from byte `at` (2-byte aligned) of a staged row on
   __device__ static __forceinline__ void words(const uint8_t *row, int at, uint32_t (&out)[8]) {
     const uint8_t *a = row + (at & ~15);
@@ -208,14 +221,15 @@ template <> struct Lane<kQ6_K> {
     for (int i = 0; i < 4; i++) {
       const float v = __fmul_rn(df, (float)s[i]);
       d[i] = f2_pack(v, v);
+      c[i] = scale_offset<32>(v);
     }
   }
   __device__ __forceinline__ void chunks(int w, uint32_t (&lo)[4], uint32_t (&hi)[4]) const {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       const uint32_t l = ql[2 * w + i], h = qh[2 * w + i];
-      scale_word<32>((l & 0x0f0f0f0fu) | ((h << 4) & 0x30303030u), d[w >> 1], lo[2 * i], lo[2 * i + 1]);
-      scale_word<32>(((l >> 4) & 0x0f0f0f0fu) | (h & 0x30303030u), d[2 + (w >> 1)], hi[2 * i], hi[2 * i + 1]);
+      scale_word<32>((l & 0x0f0f0f0fu) | ((h << 4) & 0x30303030u), d[w >> 1], c[w >> 1], lo[2 * i], lo[2 * i + 1]);
+      scale_word<32>(((l >> 4) & 0x0f0f0f0fu) | (h & 0x30303030u), d[2 + (w >> 1)], c[2 + (w >> 1)], hi[2 * i], hi[2 * i + 1]);
     }
   }
   __device__ static __forceinline__ int x_place(int c) {
@@ -227,7 +241,7 @@ template <> struct Lane<kQ6_K> {
 // element order.
 template <int TYPE> struct LaneBlocks {
   uint32_t q[16];
-  uint64_t d[2];
+  uint64_t d[2], c[2];
   __device__ __forceinline__ void fetch(const uint8_t *row, int, int t) {
     constexpr int QW = TYPE == kQ8_0 ? 8 : 4;   // words of quants in a block
     const uint8_t *a = row + (2 * QW + 1) * 4 * t;  // two blocks of 2 + 4 QW bytes
@@ -237,6 +251,8 @@ template <int TYPE> struct LaneBlocks {
     const float d0 = half_bits(w[0] & 0xffffu), d1 = half_bits(w[QW] >> 16);
     d[0] = f2_pack(d0, d0);
     d[1] = f2_pack(d1, d1);
+    c[0] = scale_offset<128>(d0);
+    c[1] = scale_offset<128>(d1);
 #pragma unroll
     for (int i = 0; i < QW; i++) {
       const uint32_t v0 = __funnelshift_r(w[i], w[i + 1], 16), v1 = w[QW + 1 + i];
@@ -256,8 +272,8 @@ template <int TYPE> struct LaneBlocks {
   __device__ __forceinline__ void chunks(int w, uint32_t (&lo)[4], uint32_t (&hi)[4]) const {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      scale_word<128>(q[2 * w + i], d[0], lo[2 * i], lo[2 * i + 1]);
-      scale_word<128>(q[8 + 2 * w + i], d[1], hi[2 * i], hi[2 * i + 1]);
+      scale_word<128>(q[2 * w + i], d[0], c[0], lo[2 * i], lo[2 * i + 1]);
+      scale_word<128>(q[8 + 2 * w + i], d[1], c[1], hi[2 * i], hi[2 * i + 1]);
     }
   }
   __device__ static __forceinline__ int x_place(int c) { return 4 * (c & 7) + (c >> 3); }
@@ -267,14 +283,14 @@ template <> struct Lane<kIQ4_NL> : LaneBlocks<kIQ4_NL> {};
 
 // The sums of a CTA's tile, left by its warps as [token][A row] f32 (rows kRows + 4 floats apart) in the idle
 // ring, to its outputs, together with the other parts' of its cluster.
-template <int NT, int kRows, bool GLU>
+template <int kTokens, int kRows, bool GLU, int kThreads>
 __device__ __forceinline__ void finish_rows(const RowsParams &p, const float *part, int m0, int n0, int parts, int rank) {
-  constexpr int kTokens = 8 * NT, kOuts = GLU ? kRows / 2 : kRows;
+  constexpr int kOuts = GLU ? kRows / 2 : kRows;
   if (parts > 1) split_sync();
   else __syncthreads();
   const int live = min(kTokens, p.m_rows - m0);
   constexpr int kQuads = kOuts / 4;
-  for (int i = rank * kRowThreads + threadIdx.x; i < live * kQuads; i += parts * kRowThreads) {
+  for (int i = rank * kThreads + threadIdx.x; i < live * kQuads; i += parts * kThreads) {
     const int token = i / kQuads, o = 4 * (i % kQuads);
     const int row = GLU ? 16 * (o >> 3) + (o & 7) : o;
     const uint32_t at = smem_u32(part + token * (kRows + 4) + row);
@@ -426,7 +442,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
 
   float *part = reinterpret_cast<float *>(smem);
   leave_tile<NT, kRowTile>(acc, part, 16 * warp + g, t);
-  finish_rows<NT, kRowTile, GLU>(p, part, m0, n0, parts, rank);
+  finish_rows<kTokens, kRowTile, GLU, kRowThreads>(p, part, m0, n0, parts, rank);
 }
 
 // The kernel's parameters but for the split, and the weights' tensor maps (gate or only matrix, up matrix); `outs`: its
@@ -460,7 +476,11 @@ template <int TYPE, bool GLU> int rows_params(const RowsCall &c, int box_row, in
 typedef void (*RowsKernel)(CUtensorMap, CUtensorMap, RowsParams);
 
 // Opts into the shared memory, once per device; `once` is the caller's, one per kernel.
-struct RowsOnce { bool configured[64]; int sms[64]; };
+struct RowsOnce {
+  bool configured[64];
+  int sms[64];
+  std::atomic<int> clusters[64][9];  // 1 + how many clusters of that many CTAs run at once
+};
 inline int rows_configure(RowsOnce &once, const void *kernel, int smem, int &sms) {
   int dev = 0;
   cudaGetDevice(&dev);
@@ -479,29 +499,58 @@ inline int rows_configure(RowsOnce &once, const void *kernel, int smem, int &sms
 // gemm_prefill.cuh).
 inline float rows_gain(int nsb) { return 1.f + 16.f * (float)nsb * 1.4901161e-8f; }
 
+inline int rows_clusters(RowsOnce &once, RowsKernel kernel, int threads, int smem, int parts) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return 0;
+  std::atomic<int> &slot = once.clusters[dev][parts];
+  int v = slot.load();
+  if (v == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, 1, parts);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = parts;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 0) {
+      cudaGetLastError();  // not cut into that many then
+      n = 0;
+    }
+    v = n + 1;
+    slot.store(v);
+  }
+  return v - 1;
+}
+
 // Chooses the split along K and launches.
-inline int rows_launch(RowsKernel kernel, RowsParams &p, const CUtensorMap (&maps)[2], int outs, int tokens, int smem, int sms,
-                       cudaStream_t s) {
+inline int rows_launch(RowsOnce &once, RowsKernel kernel, RowsParams &p, const CUtensorMap (&maps)[2], int outs, int tokens, int threads, int smem,
+                       int sms, cudaStream_t s) {
   const int blocks = (p.n_out + outs - 1) / outs, tiles = (p.m_rows + tokens - 1) / tokens;
-  // Parts of K: the SMs with the most CTAs set the time, each CTA its superblocks and a start and an end.
+  // Parts of K.  Clusters of n CTAs come in waves of as many as fit the GPU, two CTAs an SM; a CTA takes its superblocks
+  // and a start and an end, beside another one not twice as long as alone.
   int parts = 1;
   double best = 1e30;
   for (int n = 1; n <= 8 && n <= p.nsb; n++) {
     const int per = (p.nsb + n - 1) / n;
     if ((n - 1) * per >= p.nsb) continue;  // a part would be empty
-    const long long per_sm = ((long long)blocks * tiles * n + sms - 1) / sms;
-    const double cost = (per_sm < 2 ? 1.6 : per_sm) * (per + 0.5) + 2.0;
+    const int at_once = rows_clusters(once, kernel, threads, smem, n);
+    if (at_once == 0) continue;
+    const long long clusters = (long long)blocks * tiles, rest = clusters % at_once * n;  // CTAs of the last wave
+    const double load = clusters / at_once * 2.0 + (rest == 0 ? 0.0 : rest <= sms ? 1.3 : 2.0);
+    const double cost = load * (per + 0.75) + (n > 1 ? 0.5 : 0.0);
     if (cost < best) { best = cost; parts = n; }
   }
-#ifdef ROWS_TUNE
-  if (getenv("ROWS_PARTS")) parts = atoi(getenv("ROWS_PARTS"));
-#endif
   p.per = (p.nsb + parts - 1) / parts;
   parts = (p.nsb + p.per - 1) / p.per;
   p.gain = rows_gain(p.per);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks, tiles, parts);
-  cfg.blockDim = dim3(kRowThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -523,17 +572,21 @@ template <int TYPE, int NT, bool GLU, bool STAGED> int launch_rows_tile(const Ro
   constexpr int outs = GLU ? kRowTile / 2 : kRowTile;
   if (!st) st = rows_params<TYPE, GLU>(c, STAGED ? RowCfg<TYPE>::RS : 0, outs, p, maps);
   if (st) return st;
-  return rows_launch(gemm_rows_kernel<TYPE, NT, GLU, STAGED>, p, maps, outs, 8 * NT, row_smem<TYPE, NT>(), sms, s);
+  return rows_launch(once, gemm_rows_kernel<TYPE, NT, GLU, STAGED>, p, maps, outs, 8 * NT, kRowThreads, row_smem<TYPE, NT>(), sms, s);
 }
 
 template <int TYPE, bool GLU, bool STAGED> int launch_rows_width(const RowsCall &c, cudaStream_t s) {
-  // the narrowest tile that holds all rows
-  if (c.m_rows <= 8) return launch_rows_tile<TYPE, 1, GLU, STAGED>(c, s);
+  // the narrowest tile that holds all rows (rows_kernel_takes; glu_sums.cuh has up to eight of gated Q4_K / Q5_K)
+  if constexpr (!(GLU && (TYPE == kQ4_K || TYPE == kQ5_K))) {
+    if (c.m_rows <= 8) return launch_rows_tile<TYPE, 1, GLU, STAGED>(c, s);
+  }
   if (c.m_rows <= 16) return launch_rows_tile<TYPE, 2, GLU, STAGED>(c, s);
   if (c.m_rows <= 24) return launch_rows_tile<TYPE, 3, GLU, STAGED>(c, s);
-  if (c.m_rows <= 32) return launch_rows_tile<TYPE, 4, GLU, STAGED>(c, s);
-  if (c.m_rows <= 48) return launch_rows_tile<TYPE, 6, GLU, STAGED>(c, s);
-  return launch_rows_tile<TYPE, 8, GLU, STAGED>(c, s);
+  if constexpr (TYPE == kQ6_K || TYPE == kQ8_0) {
+    if (c.m_rows > 48) return launch_rows_tile<TYPE, 8, GLU, STAGED>(c, s);
+    if (c.m_rows > 32) return launch_rows_tile<TYPE, 6, GLU, STAGED>(c, s);
+  }
+  return launch_rows_tile<TYPE, 4, GLU, STAGED>(c, s);
 }
 
 template <bool GLU> int launch_rows(const RowsCall &c, cudaStream_t s) {

@@ -1,14 +1,9 @@
-// The plain form of the product for few rows (rows_stream.cuh, gemm_rows.cuh).
-#include <cstdlib>
-
-#include "rows_stream.cuh"
+// The plain form of the product for few rows (gemm_rows.cuh).
+#include "gemm_rows.cuh"
 
 namespace cogni {
 
-int launch_gemm_rows_epilogue(const RowsCall &c, cudaStream_t s) {
-  const int st = launch_rows_stream<false>(c, s);
-  return st == kNotTaken ? launch_rows<false>(c, s) : st;
-}
+int launch_gemm_rows_epilogue(const RowsCall &c, cudaStream_t s) { return launch_rows<false>(c, s); }
 unsigned gemm_rows_epilogue_timeouts() { return rows_timeouts(); }
 int gemm_rows_epilogue_reset_timeouts() { return rows_reset_timeouts(); }
 

@@ -72,28 +72,25 @@ __device__ __forceinline__ void store1(void *p, bool bf16, long long at, float v
 template <bool VEC> __device__ __forceinline__ int place(int c, int i) {
   return VEC ? 8 * ((int)blockDim.x * c + (int)threadIdx.x) + i : (int)blockDim.x * (8 * c + i) + (int)threadIdx.x;
 }
-// `live`: the elements of chunk c that lie in the row, from the first on
-template <bool VEC> __device__ __forceinline__ int live(int c, int n) {
-  if (VEC) return place<true>(c, 0) < n ? 8 : 0;  // n is a multiple of eight
-  const int left = n - place<false>(c, 0);
-  return left <= 0 ? 0 : min(8, (left + (int)blockDim.x - 1) / (int)blockDim.x);
-}
-template <bool VEC> __device__ __forceinline__ void load_chunk(const void *p, bool bf16, long long row, int c, int cnt, float (&v)[8]) {
+// whether element i of chunk c lies in the row (VEC: n is a multiple of eight, a chunk does or does not)
+template <bool VEC> __device__ __forceinline__ bool inside(int c, int i, int n) { return place<VEC>(c, VEC ? 0 : i) < n; }
+
+template <bool VEC> __device__ __forceinline__ void load_chunk(const void *p, bool bf16, long long row, int c, int n, float (&v)[8]) {
   if (VEC) {
-    if (cnt) load8(p, bf16, row + place<true>(c, 0), v);
+    if (inside<true>(c, 0, n)) load8(p, bf16, row + place<true>(c, 0), v);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++)
-      if (i < cnt) v[i] = load1(p, bf16, row + place<false>(c, i));
+      if (inside<false>(c, i, n)) v[i] = load1(p, bf16, row + place<false>(c, i));
   }
 }
-template <bool VEC> __device__ __forceinline__ void store_chunk(void *p, bool bf16, long long row, int c, int cnt, const float (&v)[8]) {
+template <bool VEC> __device__ __forceinline__ void store_chunk(void *p, bool bf16, long long row, int c, int n, const float (&v)[8]) {
   if (VEC) {
-    if (cnt) store8(p, bf16, row + place<true>(c, 0), v);
+    if (inside<true>(c, 0, n)) store8(p, bf16, row + place<true>(c, 0), v);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++)
-      if (i < cnt) store1(p, bf16, row + place<false>(c, i), v[i]);
+      if (inside<false>(c, i, n)) store1(p, bf16, row + place<false>(c, i), v[i]);
   }
 }
 
@@ -116,16 +113,13 @@ __device__ __forceinline__ float row_sum(float v, float *slots, int &turn) {
 
 template <int C, bool VEC>
 __device__ __forceinline__ void normalise(const NormSide &s, float (&v)[C][8], int n, float *slots, int &turn) {
-  int cnt[C];
   float sum = 0.f, inv_n = 1.f / (float)n;
-#pragma unroll
-  for (int c = 0; c < C; c++) cnt[c] = live<VEC>(c, n);
   if (s.layer) {
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        if (i < cnt[c]) sum += v[c][i];
+        if (inside<VEC>(c, i, n)) sum += v[c][i];
     const float mean = row_sum(sum, slots, turn) * inv_n;
 #pragma unroll
     for (int c = 0; c < C; c++)
@@ -137,36 +131,36 @@ __device__ __forceinline__ void normalise(const NormSide &s, float (&v)[C][8], i
   for (int c = 0; c < C; c++)
 #pragma unroll
     for (int i = 0; i < 8; i++)
-      if (i < cnt[c]) sum += v[c][i] * v[c][i];
+      if (inside<VEC>(c, i, n)) sum += v[c][i] * v[c][i];
   const float r = rsqrtf(row_sum(sum, slots, turn) * inv_n + s.eps);
 #pragma unroll
   for (int c = 0; c < C; c++) {
     float w[8];
-    load_chunk<VEC>(s.w, false, 0, c, cnt[c], w);
+    load_chunk<VEC>(s.w, false, 0, c, n, w);
 #pragma unroll
     for (int i = 0; i < 8; i++) v[c][i] = v[c][i] * r * w[i];
     if (s.b) {
-      load_chunk<VEC>(s.b, false, 0, c, cnt[c], w);
+      load_chunk<VEC>(s.b, false, 0, c, n, w);
 #pragma unroll
       for (int i = 0; i < 8; i++) v[c][i] += w[i];
     }
   }
 }
 
+// Full occupancy (32 registers) for the vector form of one chunk: 4096 rows x 5120 with both norms 63 us at 40 registers,
+// 58 at 32.  (Tried and slower: the rows past the L1, 62; the next row loaded beside this one's reductions, 76.)
 template <int C, bool VEC>
-__global__ void __launch_bounds__(1024) norm_residual_kernel(const NormParams p) {
+__global__ void __launch_bounds__(1024, C == 1 && VEC ? 2 : 1) norm_residual_kernel(const NormParams p) {
   __shared__ float slots[64];
   int turn = 0;
   const long long m = blockIdx.x;
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   float h[C][8], b[C][8];
-  int cnt[C];
 #pragma unroll
   for (int c = 0; c < C; c++) {
-    cnt[c] = live<VEC>(c, p.n);
-    if (p.block) load_chunk<VEC>(p.block, p.block_bf16, m * p.block_stride, c, cnt[c], b[c]);
-    load_chunk<VEC>(p.residual, p.residual_bf16, m * p.residual_stride, c, cnt[c], h[c]);
+    if (p.block) load_chunk<VEC>(p.block, p.block_bf16, m * p.block_stride, c, p.n, b[c]);
+    load_chunk<VEC>(p.residual, p.residual_bf16, m * p.residual_stride, c, p.n, h[c]);
   }
   if (p.block) {
     if (p.post.w) normalise<C, VEC>(p.post, b, p.n, slots, turn);
@@ -174,7 +168,7 @@ __global__ void __launch_bounds__(1024) norm_residual_kernel(const NormParams p)
     for (int c = 0; c < C; c++) {
       if (p.gate) {
         float g[8];
-        load_chunk<VEC>(p.gate, p.gate_bf16, m * p.gate_stride, c, cnt[c], g);
+        load_chunk<VEC>(p.gate, p.gate_bf16, m * p.gate_stride, c, p.n, g);
 #pragma unroll
         for (int i = 0; i < 8; i++) b[c][i] *= g[i];
       }
@@ -184,12 +178,12 @@ __global__ void __launch_bounds__(1024) norm_residual_kernel(const NormParams p)
   }
   if (p.h) {
 #pragma unroll
-    for (int c = 0; c < C; c++) store_chunk<VEC>(p.h, p.h_bf16, m * p.h_stride, c, cnt[c], h[c]);
+    for (int c = 0; c < C; c++) store_chunk<VEC>(p.h, p.h_bf16, m * p.h_stride, c, p.n, h[c]);
   }
   if (p.pre.w) {
     normalise<C, VEC>(p.pre, h, p.n, slots, turn);
 #pragma unroll
-    for (int c = 0; c < C; c++) store_chunk<VEC>(p.y, p.y_bf16, m * p.y_stride, c, cnt[c], h[c]);
+    for (int c = 0; c < C; c++) store_chunk<VEC>(p.y, p.y_bf16, m * p.y_stride, c, p.n, h[c]);
   }
 }
 

@@ -146,7 +146,12 @@ struct RowsCall {
   RowEpilogue epi;
 };
 
-// Few rows go to the kernel that streams the weights (gemm_rows.cuh), more to the tensor-core tiles.
-inline bool rows_kernel_takes(const RowsCall &c) { return c.m_rows <= 64; }
+// Few rows go to the kernels that expand weights in registers (gemm_rows.cuh, glu_sums.cuh), more to the tensor-core tiles
+// (gemm_prefill.cuh), whose expansion into shared memory does not get dearer with the tokens but is slow for Q6_K and Q8_0.
+// Over 6183 drawn shapes, time of the first over that of the best tile, geometric means at 25-32 / 41-48 / 57-64 rows: Q4_K
+// 0.96 / 1.12 / 1.3, Q5_K 0.97 / 1.05 / 1.5, IQ4_NL 0.88 / 1.13 / 1.3, Q8_0 0.57 / 0.74 / 0.87, Q6_K 0.49 / 0.68 / 0.80.
+inline bool rows_kernel_takes(const RowsCall &c) {
+  return c.m_rows <= (c.type == COGNI_QMM_TYPE_Q6_K || c.type == COGNI_QMM_TYPE_Q8_0 ? 64 : 32);
+}
 
 }  // namespace cogni

@@ -9,7 +9,7 @@ from typing import Optional
 import torch
 
 from ._lib import lib
-from .quant_matmul import _call, _output, _row_type, _rows, _vector
+from .quant_matmul import _ROW_TYPE, _call, _output, _row_type, _rows, _vector
 
 _KINDS = {"rms": 0, "layer": 1}
 _NORM_ARGS = struct.Struct("5Q5q2Qfi2Qfi5if2i")  # cogni_qmm_norm_args
@@ -46,43 +46,49 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
     dev = residual.get_device()
     if dev < 0:
         raise ValueError("residual must be on a CUDA device")
-    m, res_stride = _rows(residual, n, "residual")
-    if block is None and norm is None:
-        raise ValueError("nothing to compute: neither block nor norm")
+    m, res_stride = _rows(residual, n, dev, "residual")
+    res_type = _row_type(residual, "residual")
 
     def side(t, name):
-        rows, stride = _rows(t, n, name)
-        if rows != m or t.get_device() != dev:
-            raise ValueError(f"{name} must have a row for every row of residual, on its device")
+        rows, stride = _rows(t, n, dev, name)
+        if rows != m:
+            raise ValueError(f"{name} must have a row for every row of residual")
         return t.data_ptr(), stride, _row_type(t, name)
 
-    block_ptr, block_stride, block_type = side(block, "block") if block is not None else (0, 0, 0)
-    gate_ptr = gate_stride = gate_type = 0
-    if block is None:
-        if post_norm is not None or gate is not None:
-            raise ValueError("post_norm and gate belong to a block")
-    elif gate is not None:
-        if gate.dim() == 1 or (gate.numel() == n and m != 1):
-            if gate.numel() != n or not gate.is_contiguous() or gate.get_device() != dev:
-                raise ValueError(f"gate must have {n} contiguous elements, or a row for every row of residual")
-            gate_ptr, gate_type = gate.data_ptr(), _row_type(gate, "gate")
-        else:
-            gate_ptr, gate_stride, gate_type = side(gate, "gate")
-    if hidden is None and block is not None:
-        hidden = _output(m, n, residual, residual.dtype, dev, stream)
-    h_ptr, h_stride, h_type = side(hidden, "hidden") if hidden is not None else (0, 0, 0)
+    block_ptr = block_stride = block_type = gate_ptr = gate_stride = gate_type = 0
+    if block is not None:
+        block_ptr, block_stride, block_type = side(block, "block")
+        if gate is not None:
+            if gate.numel() == n:  # one row for all
+                if not gate.is_contiguous() or gate.get_device() != dev:
+                    raise ValueError(f"gate must have {n} contiguous elements, or a row for every row of residual")
+                gate_ptr, gate_type = gate.data_ptr(), _row_type(gate, "gate")
+            else:
+                gate_ptr, gate_stride, gate_type = side(gate, "gate")
+    elif post_norm is not None or gate is not None:
+        raise ValueError("post_norm and gate belong to a block")
+    elif norm is None:
+        raise ValueError("nothing to compute: neither block nor norm")
+    h_ptr = h_stride = h_type = 0
+    if hidden is not None:
+        h_ptr, h_stride, h_type = side(hidden, "hidden")
+    elif block is not None:
+        hidden = _output(residual, n, residual.dtype, stream)
+        h_ptr, h_stride, h_type = hidden.data_ptr(), n, res_type
     y_ptr = y_stride = y_type = 0
     if norm is not None:
         if out is None:
-            out = _output(m, n, residual, out_dtype, dev, stream)
-        y_ptr, y_stride, y_type = side(out, "out")
+            out = _output(residual, n, out_dtype, stream)
+            y_ptr, y_stride, y_type = out.data_ptr(), n, _ROW_TYPE[out_dtype]
+        else:
+            y_ptr, y_stride, y_type = side(out, "out")
     elif out is not None:
         raise ValueError("out is the result of norm")
-    args = (residual.data_ptr(), block_ptr, gate_ptr, h_ptr, y_ptr,
-            res_stride, block_stride, gate_stride, h_stride, y_stride,
-            *(post_norm._fields(n, dev) if post_norm is not None else _NO_NORM),
-            *(norm._fields(n, dev) if norm is not None else _NO_NORM),
-            _row_type(residual, "residual"), block_type, gate_type, h_type, y_type, scale, m, n)
+    args = _NORM_ARGS.pack(residual.data_ptr(), block_ptr, gate_ptr, h_ptr, y_ptr,
+                           res_stride, block_stride, gate_stride, h_stride, y_stride,
+                           *(post_norm._fields(n, dev) if post_norm is not None else _NO_NORM),
+                           *(norm._fields(n, dev) if norm is not None else _NO_NORM),
+                           res_type, block_type, gate_type, h_type, y_type, scale, m, n)
     if m:
-        _call(lib.cogni_qmm_norm_residual, "cogni_qmm_norm_residual", _NORM_ARGS.pack(*args), dev, stream)
+        _call(lib.cogni_qmm_norm_residual, "cogni_qmm_norm_residual", args, dev, stream)
     return hidden if hidden is not None else residual, out

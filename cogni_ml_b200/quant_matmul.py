@@ -306,10 +306,12 @@ _ROW_TYPE = {torch.float32: 0, torch.bfloat16: 1}
 _GEMM_ARGS = struct.Struct("7Q3q8i")  # cogni_qmm_gemm_args
 
 
-def _rows(t: torch.Tensor, width: int, name: str):
-    """(rows, elements between rows) of a tensor whose last dimension has `width` elements."""
-    if t.shape[-1] != width:
-        raise ValueError(f"{name} must have {width} columns, got shape {tuple(t.shape)}")
+# These checks run on every call, a few microseconds that small calls are bound by: plain attribute reads, no
+# objects made on the way.
+def _rows(t: torch.Tensor, width: int, dev: int, name: str):
+    """(rows, elements between rows) of a tensor on device `dev` whose last dimension has `width` elements."""
+    if t.get_device() != dev or t.shape[-1] != width:
+        raise ValueError(f"{name} must have {width} columns and be on device {dev}, got shape {tuple(t.shape)} on {t.device}")
     if t.is_contiguous():
         return t.numel() // width, width
     if t.dim() == 2 and t.stride(1) == 1:
@@ -328,25 +330,31 @@ def _vector(t: Optional[torch.Tensor], n: int, dev: int, name: str) -> int:
     """Address of an f32 [n] vector on device `dev`, 0 for None."""
     if t is None:
         return 0
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
+    if t.dtype is not torch.float32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous f32 tensor of {n} elements on the device of the rows")
     return t.data_ptr()
 
 
 def _call(fn, what: str, args: bytes, dev: int, stream) -> None:
-    """Launches on device `dev`, whatever device is current."""
-    if dev == torch.cuda.current_device():
-        check(fn(args, _stream_ptr(stream)), what)
+    """Launches on device `dev`, whatever device is current, on `stream` or that device's current one."""
+    handle = stream.cuda_stream if stream else torch._C._cuda_getCurrentRawStream(dev)
+    if torch._C._cuda_getDevice() == dev:
+        status = fn(args, handle)
     else:
         with torch.cuda.device(dev):
-            check(fn(args, _stream_ptr(stream)), what)
+            status = fn(args, handle)
+    if status:
+        check(status, what)
 
 
-def _output(rows: int, width: int, like: torch.Tensor, dtype, dev: int, stream) -> torch.Tensor:
+def _output(like: torch.Tensor, width: int, dtype, stream) -> torch.Tensor:
+    """A new tensor with the rows of `like`, `width` columns and the given type."""
     if dtype not in _ROW_TYPE:
         raise ValueError(f"outputs are f32 or bf16, not {dtype}")
-    shape = (rows, width) if like.dim() == 2 else like.shape[:-1] + (width,)
-    out = torch.empty(shape, dtype=dtype, device=like.device)
+    if like.shape[-1] == width and like.is_contiguous():
+        out = torch.empty_like(like) if like.dtype is dtype else torch.empty_like(like, dtype=dtype)
+    else:
+        out = like.new_empty(like.shape[:-1] + (width,), dtype=dtype)
     if stream:  # allocated on the current stream, written on another
         out.record_stream(stream)
     return out
@@ -354,39 +362,40 @@ def _output(rows: int, width: int, like: torch.Tensor, dtype, dev: int, stream) 
 
 def _gemm_rows(w: DeviceQuantWeight, up: Optional[DeviceQuantWeight], x, bias, bias_up, activation, residual,
                out_dtype, out, stream) -> torch.Tensor:
-    n, k = w.out_dim, w.in_dim
-    dev = x.get_device()
-    if x.dtype != torch.bfloat16 or dev < 0 or w.raw.get_device() != dev:
+    n, k, raw = w.out_dim, w.in_dim, w.raw
+    dev = raw.get_device()
+    if dev < 0 or x.get_device() != dev or x.dtype is not torch.bfloat16:
         raise ValueError("x must be a bf16 tensor on the device of the weights")
     act = _ACT_CODE.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {ACTIVATIONS}, got {activation!r}")
-    m, x_stride = _rows(x, k, "x")
-    if up is not None and ((up.type, up.out_dim, up.in_dim) != (w.type, n, k) or up.raw.get_device() != dev):
-        raise ValueError("gate and up must have the same type, shape and device")
+    m, x_stride = _rows(x, k, dev, "x")
+    up_ptr, resident = 0, w.resident
+    if up is not None:
+        if up.type != w.type or up.out_dim != n or up.in_dim != k or up.raw.get_device() != dev:
+            raise ValueError("gate and up must have the same type, shape and device")
+        up_ptr, resident = up.raw.data_ptr(), resident and up.resident
     res_ptr = res_stride = res_type = 0
     if residual is not None:
-        res_m, res_stride = _rows(residual, n, "residual")
-        if res_m != m or residual.get_device() != dev:
-            raise ValueError("residual must have a row for every row of x, on its device")
+        res_m, res_stride = _rows(residual, n, dev, "residual")
+        if res_m != m:
+            raise ValueError("residual must have a row for every row of x")
         res_ptr, res_type = residual.data_ptr(), _row_type(residual, "residual")
+    y_stride = n
     if out is None:
-        out = _output(m, n, x, out_dtype, dev, stream)
-        y_stride = n
+        out = _output(residual if residual is not None and residual.dim() == x.dim() else x, n, out_dtype, stream)
     else:
-        out_m, y_stride = _rows(out, n, "out")
-        if out_m != m or out.get_device() != dev:
-            raise ValueError("out must have a row for every row of x, on its device")
-    y_type = _row_type(out, "out")
-    args = (w.raw.data_ptr(), up.raw.data_ptr() if up is not None else 0, x.data_ptr(), _vector(bias, n, dev, "bias"),
-            _vector(bias_up, n, dev, "bias_up"), res_ptr, out.data_ptr(), x_stride, res_stride, y_stride, w.type, act,
-            res_type, y_type, m, n, k, 1 if w.resident and (up is None or up.resident) else 0)
-    if m == 0:
-        return out
-    if up is None:
-        _call(lib.cogni_qmm_gemm_epilogue, "cogni_qmm_gemm_epilogue", _GEMM_ARGS.pack(*args), dev, stream)
-    else:
-        _call(lib.cogni_qmm_gemm_glu, "cogni_qmm_gemm_glu", _GEMM_ARGS.pack(*args), dev, stream)
+        out_m, y_stride = _rows(out, n, dev, "out")
+        if out_m != m:
+            raise ValueError("out must have a row for every row of x")
+    args = _GEMM_ARGS.pack(raw.data_ptr(), up_ptr, x.data_ptr(), _vector(bias, n, dev, "bias"),
+                           _vector(bias_up, n, dev, "bias_up"), res_ptr, out.data_ptr(), x_stride, res_stride, y_stride,
+                           w.type, act, res_type, _row_type(out, "out"), m, n, k, resident)
+    if m:
+        if up is None:
+            _call(lib.cogni_qmm_gemm_epilogue, "cogni_qmm_gemm_epilogue", args, dev, stream)
+        else:
+            _call(lib.cogni_qmm_gemm_glu, "cogni_qmm_gemm_glu", args, dev, stream)
     return out
 
 

@@ -317,6 +317,43 @@ module ML::CUDA
         "cogni_qmm_gemm_bf16"
     end
 
+    # y[m, :] = residual[m, :] + act(W x[m, :] + bias) for any number of rows; residual f32 or bf16 as y.
+    def gemm_epilogue(x_bf16 : DeviceBuffer, y : DeviceBuffer, m_rows : Int32, out_bf16 : Bool = false,
+                      activation : Int32 = LibCogniQMM::ACT_NONE, bias : DeviceBuffer? = nil,
+                      residual : DeviceBuffer? = nil, stream : Void* = ML::CUDA.current_stream) : Nil
+      args = rows_args(x_bf16, y, m_rows, out_bf16, activation)
+      args.bias = bias ? bias.ptr : 0_u64
+      args.residual = residual ? residual.ptr : 0_u64
+      args.residual_stride = @out_dim.to_i64
+      args.residual_type = args.y_type
+      ML::CUDA.qmm_check! LibCogniQMM.cogni_qmm_gemm_epilogue(pointerof(args), stream), "cogni_qmm_gemm_epilogue"
+    end
+
+    # y[m, :] = act(gate x[m, :]) * (up x[m, :]) as bf16; self is the gate.
+    def gemm_glu(up : DeviceQuantWeight, x_bf16 : DeviceBuffer, y_bf16 : DeviceBuffer, m_rows : Int32,
+                 activation : Int32 = LibCogniQMM::ACT_SILU, stream : Void* = ML::CUDA.current_stream) : Nil
+      args = rows_args(x_bf16, y_bf16, m_rows, true, activation)
+      args.w_up = up.buffer.ptr
+      ML::CUDA.qmm_check! LibCogniQMM.cogni_qmm_gemm_glu(pointerof(args), stream), "cogni_qmm_gemm_glu"
+    end
+
+    private def rows_args(x : DeviceBuffer, y : DeviceBuffer, m_rows : Int32, out_bf16 : Bool, activation : Int32)
+      args = LibCogniQMM::GemmArgs.new
+      args.w = @buffer.ptr
+      args.x = x.ptr
+      args.y = y.ptr
+      args.x_stride = @in_dim.to_i64
+      args.y_stride = @out_dim.to_i64
+      args.type = @type.value.to_i32
+      args.activation = activation
+      args.y_type = out_bf16 ? LibCogniQMM::OUT_BF16 : LibCogniQMM::OUT_F32
+      args.m_rows = m_rows
+      args.n_out = @out_dim
+      args.k_in = @in_dim
+      args.resident = 1
+      args
+    end
+
     def close : Nil
       return if @closed
       @top1_scratch.try &.close

@@ -120,6 +120,45 @@ struct DeviceQuantWeight {
                               in_dim, stream),
           "cogni_qmm_gemm_bf16");
   }
+  // y[m, :] = residual[m, :] + act(W x[m, :] + bias), any number of rows, contiguous; residual of y's type
+  void gemm_epilogue(const void *d_x_bf16, void *d_y, int m_rows, int out_type = COGNI_QMM_OUT_F32,
+                     int activation = COGNI_QMM_ACT_NONE, const float *d_bias = nullptr, const void *d_residual = nullptr,
+                     void *stream = nullptr) const {
+    cogni_qmm_gemm_args a = rows_args(d_x_bf16, d_y, m_rows, out_type, activation);
+    a.bias = d_bias;
+    a.residual = d_residual;
+    a.residual_stride = out_dim;
+    a.residual_type = out_type;
+    check(cogni_qmm_gemm_epilogue(&a, stream), "cogni_qmm_gemm_epilogue");
+  }
+  // y[m, :] = act(W x[m, :]) * (up x[m, :]) as bf16; this weight is the gate
+  void gemm_glu(const DeviceQuantWeight &up, const void *d_x_bf16, void *d_y_bf16, int m_rows,
+                int activation = COGNI_QMM_ACT_SILU, void *stream = nullptr) const {
+    if (up.type != type || up.out_dim != out_dim || up.in_dim != in_dim)
+      throw std::invalid_argument("gate and up must have the same type and shape");
+    cogni_qmm_gemm_args a = rows_args(d_x_bf16, d_y_bf16, m_rows, COGNI_QMM_OUT_BF16, activation);
+    a.w_up = up.d_raw;
+    a.resident = resident && up.resident;
+    check(cogni_qmm_gemm_glu(&a, stream), "cogni_qmm_gemm_glu");
+  }
+
+ private:
+  cogni_qmm_gemm_args rows_args(const void *d_x, void *d_y, int m_rows, int out_type, int activation) const {
+    cogni_qmm_gemm_args a = {};
+    a.w = d_raw;
+    a.x = d_x;
+    a.y = d_y;
+    a.x_stride = in_dim;
+    a.y_stride = out_dim;
+    a.type = static_cast<int>(type);
+    a.activation = activation;
+    a.y_type = out_type;
+    a.m_rows = m_rows;
+    a.n_out = out_dim;
+    a.k_in = in_dim;
+    a.resident = resident ? 1 : 0;
+    return a;
+  }
 };
 
 }  // namespace cogni_qmm

@@ -96,7 +96,9 @@ def healthy(engine):
 # row counts around every boundary of the kernels' tiles, and a few prompt-sized ones
 SHAPES = [(1, 64, 256), (1, 2053, 1024), (2, 300, 768), (7, 129, 512), (8, 1000, 2048), (9, 16, 256), (15, 128, 1280),
           (16, 256, 4096), (17, 515, 512), (31, 33, 1024), (33, 130, 256), (63, 513, 768), (64, 384, 2048), (65, 200, 1536),
-          (100, 96, 512), (127, 260, 256), (130, 1111, 512), (300, 257, 1024), (700, 300, 512), (1100, 640, 256)]
+          (100, 96, 512), (127, 260, 256), (130, 1111, 512), (300, 257, 1024), (700, 300, 512), (1100, 640, 256),
+          # enough rows of weights for several parts of K, waves of clusters and every kernel of the gated form
+          (3, 9000, 1024), (12, 4104, 4352), (20, 4109, 4096), (29, 6002, 3328), (90, 5003, 2048)]
 
 
 @pytest.mark.parametrize("qtype", TYPES)
@@ -124,6 +126,27 @@ def test_glu_matches_its_definition(cuda, oracle, engine, qtype, m, n, k):
         forms = [glu_reference(x, g, u, b1, b2, act) for g, u in ((wg.rounded, wu.rounded), (wg.exact, wu.exact))]
         if not any(within(y, *f) for f in forms):
             check(y, *forms[0])
+    healthy(engine)
+
+
+# cogni_qmm_set_kernel_choice: token-tile width 128 / 256 / 512, parts of K 1 / 2 / 4, the CTA pair off, direct loads
+@pytest.mark.parametrize("choices", [(49, 53), (49, 54), (49, 59), (50, 53), (50, 54), (51, 53), (51, 54), (51, 53, 58), (49, 56), (51, 56)])
+@pytest.mark.parametrize("qtype", TYPES)
+def test_every_tile_and_split(cuda, oracle, engine, choices, qtype):
+    m, n, k = 530, 200, 1024
+    w, x = inputs(cuda, oracle, qtype, m, n, k, seed=17)
+    wu = Weight(cuda, oracle, qtype, n, k, seed=18)
+    bias, residual = rows(cuda, 1, n, 5).view(-1), rows(cuda, m, n, 6)
+    for c in choices:
+        assert engine.lib.cogni_qmm_set_kernel_choice(c) == 0
+    try:
+        y = w.dev.gemm_epilogue(x, bias=bias, activation="relu", residual=residual)
+        g = gemm_glu(w.dev, wu.dev, x, bias_gate=bias)
+    finally:
+        for c in (48, 52, 55, 57):
+            engine.lib.cogni_qmm_set_kernel_choice(c)
+    check(y, *epilogue_reference(x, w, bias, "relu", residual, torch.float32))
+    check(g, *glu_reference(x, w.rounded, wu.rounded, bias, None, "silu"))
     healthy(engine)
 
 
