@@ -676,6 +676,7 @@ __device__ __forceinline__ void prefetch_residual(const GemmParams &p, int m, in
 }
 // The accumulator columns cbeg .. cbeg + cols (a multiple of 32) of the 32 TMEM lanes 32 q .. of a tile at
 // (token m0, output n0) to y: for a fixed token the lanes store consecutive outputs.
+// (kEpilogue: epilogue_tile.)
 template <int MODE>
 __device__ __forceinline__ void store_columns(const GemmParams &p, uint32_t taddr, int cbeg, int cols, int m0, int n0,
                                               int q, int lane) {
@@ -700,31 +701,6 @@ __device__ __forceinline__ void store_columns(const GemmParams &p, uint32_t tadd
         }
       }
     }
-  } else if constexpr (MODE == kEpilogue) {
-    const int n = n0 + 32 * q + lane;
-    const float bias = p.epi.bias && n < p.n_out ? __ldg(p.epi.bias + n) : 0.f;
-    with_activation(p.epi.activation, [&](auto act) {
-#pragma unroll 1
-      for (int c0 = cbeg; c0 < cbeg + cols && m0 + c0 < p.m_rows; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld32(taddr + c0, v);
-        tmem_ld_wait();
-        if (n < p.n_out) {
-          const int live = min(32, p.m_rows - m0 - c0);
-          // the residual may be y itself: sixteen loads before the first store, so that they overlap
-#pragma unroll
-          for (int h = 0; h < 32; h += 16) {
-            float r[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) r[j] = h + j < live ? load_residual(p.epi, m0 + c0 + h + j, n) : 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; j++)
-              if (h + j < live)
-                store_out(p.epi, m0 + c0 + h + j, n, r[j] + activate<decltype(act)::value>(fmaf(p.gain, __uint_as_float(v[h + j]), bias)));
-          }
-        }
-      }
-    });
   } else {
     const int n = n0 + 16 * q + (lane & 15);
     const bool up = lane >= 16;
@@ -748,6 +724,74 @@ __device__ __forceinline__ void store_columns(const GemmParams &p, uint32_t tadd
         }
       }
     });
+  }
+}
+
+// kEpilogue, a tile that is not split: the token columns of the accumulator through the idle ring, so that a warp finishes
+// a token's 128 outputs together, four a lane: residual and y are then 512 (256) contiguous bytes an access.  Lanes
+// holding one output each, as store_columns has it, took 20 us a tile for the residual's loads alone (Q4_K
+// 12288 x 4096, 4096 tokens, f32 residual: 471 us, bf16 552; without one 394).
+//
+// finish_columns: the columns of one round (part: [column][128] f32) from token `first` on, by the CTA's warps.  A function
+// of its own: inlined into the loop over the rounds, the constants of all activations stay in registers across it (80 more).
+__device__ __noinline__ void finish_columns(const RowEpilogue e, float gain, const float *part, int first, int live, int n, int n_out) {
+  constexpr int kAhead = 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = (int)blockDim.x >> 5;
+  if (e.vec && n + 4 <= n_out) {
+    float bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) bias[i] = e.bias ? __ldg(e.bias + n + i) : 0.f;
+    with_activation(e.activation, [&](auto act) {
+#pragma unroll 1
+      for (int c = warp; c < live; c += kAhead * nw) {
+        // the residual may be y itself: the loads of four tokens before the first store, so that they overlap
+        uint4 r[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++)
+          if (c + u * nw < live) r[u] = residual4_bits(e, first + c + u * nw, n);
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          if (c + u * nw >= live) break;
+          const float4 s = *reinterpret_cast<const float4 *>(part + (c + u * nw) * kBM + 4 * lane);
+          const float v[4] = {s.x, s.y, s.z, s.w};
+          float f[4];
+          residual4_values(e, r[u], f);
+#pragma unroll
+          for (int i = 0; i < 4; i++) f[i] += activate<decltype(act)::value>(fmaf(gain, v[i], bias[i]));
+          store_out4(e, first + c + u * nw, n, f);
+        }
+      }
+    });
+  } else if (n < n_out) {
+#pragma unroll 1
+    for (int c = warp; c < live; c += nw) {
+      const float4 s = *reinterpret_cast<const float4 *>(part + c * kBM + 4 * lane);
+      const float v[4] = {gain * s.x, gain * s.y, gain * s.z, gain * s.w};
+      epilogue_store4(e, v, first + c, n, n_out);
+    }
+  }
+}
+// All threads of the CTA; `taddr`: the calling warp's lane quarter; chunk (of kChunks, -1: none): its share of the columns.
+template <int BN, int kChunks>
+__device__ __forceinline__ void epilogue_tile(const GemmParams &p, float *part, uint32_t taddr, int chunk, int m0, int n0, int q, int lane) {
+  constexpr int kRound = BN < 256 ? BN : 256, kCols = kRound / kChunks;
+  const int end = min(BN, p.m_rows - m0);
+#pragma unroll 1
+  for (int r0 = 0; r0 < end; r0 += kRound) {
+    const int live = min(kRound, end - r0);
+    if (chunk >= 0) {
+#pragma unroll 1
+      for (int c0 = chunk * kCols; c0 < (chunk + 1) * kCols && c0 < live; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld32(taddr + r0 + c0, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j++) part[(c0 + j) * kBM + 32 * q + lane] = __uint_as_float(v[j]);
+      }
+    }
+    __syncthreads();
+    finish_columns(p.epi, p.gain, part, m0 + r0, live, n0 + 4 * lane, p.n_out);
+    __syncthreads();  // the columns have been read
   }
 }
 
@@ -995,7 +1039,11 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
     tc_fence_after();
   }
   if (p.splits == 1) {
-    if (R::in_epilogue(warp)) {
+    if constexpr (MODE == kEpilogue) {
+      static_assert((BN < 256 ? BN : 256) * kBM * 4 <= kStages * kStageBytes, "a round of the tile fits the ring");
+      epilogue_tile<BN, kChunks>(p, reinterpret_cast<float *>(smem), taddr, R::in_epilogue(warp) ? R::epilogue_chunk(warp) : -1, m0,
+                                 n0, q, lane);
+    } else if (R::in_epilogue(warp)) {
       constexpr int kCols = BN / kChunks;
       store_columns<MODE>(p, taddr, R::epilogue_chunk(warp) * kCols, kCols, m0, n0, q, lane);
     }
@@ -1316,14 +1364,21 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   }
   // ---------------------------------------------------------------- epilogue (own 128 rows)
+  const int q = warp & 3;
+  const uint32_t taddr = tmem_base + ((uint32_t)(32 * q) << 16);
   if (R::in_epilogue(warp)) {
-    const int q = warp & 3;
     constexpr int kCols = kPairBN / 4;
-    const int cbeg = R::epilogue_chunk(warp) * kCols;
-    if constexpr (MODE == kEpilogue) prefetch_residual(p, m0 + cbeg, kCols, n0 + 32 * q, lane);
+    if constexpr (MODE == kEpilogue) prefetch_residual(p, m0 + R::epilogue_chunk(warp) * kCols, kCols, n0 + 32 * q, lane);
     mbar_wait(smem_u32(&bars[kAccBar]), 0);
     tc_fence_after();
-    store_columns<MODE>(p, tmem_base + ((uint32_t)(32 * q) << 16), cbeg, kCols, m0, n0, q, lane);
+    if constexpr (MODE != kEpilogue)
+      store_columns<MODE>(p, taddr, R::epilogue_chunk(warp) * kCols, kCols, m0, n0, q, lane);
+  }
+  if constexpr (MODE == kEpilogue) {
+    // the accumulator barrier follows the last MMA of both CTAs: their rings are idle
+    static_assert(256 * kBM * 4 <= kSA * kATile + kSB * kPairBStage, "a round of the tile fits the ring");
+    epilogue_tile<kPairBN, 4>(p, reinterpret_cast<float *>(smem), taddr, R::in_epilogue(warp) ? R::epilogue_chunk(warp) : -1, m0, n0, q,
+                              lane);
   }
 
   tc_fence_before();

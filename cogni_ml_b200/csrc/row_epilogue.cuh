@@ -76,21 +76,30 @@ __device__ __forceinline__ void store_out4(const RowEpilogue &e, int m, int n, c
   else
     *reinterpret_cast<float4 *>(reinterpret_cast<float *>(e.y) + at) = make_float4(f[0], f[1], f[2], f[3]);
 }
+// The residual of four outputs n .. n + 3 of row m in one access (RowEpilogue::vec), as read and as values; zero where there
+// is none.
+__device__ __forceinline__ uint4 residual4_bits(const RowEpilogue &e, int m, int n) {
+  if (!e.residual) return make_uint4(0, 0, 0, 0);
+  const long long at = (long long)m * e.residual_stride + n;
+  if (e.residual_bf16) {
+    const uint2 b = *reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(e.residual) + at);
+    return make_uint4(b.x, b.y, 0, 0);
+  }
+  return *reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(e.residual) + at);
+}
+__device__ __forceinline__ void residual4_values(const RowEpilogue &e, const uint4 &b, float (&r)[4]) {
+  r[0] = e.residual_bf16 ? bf16_value(b.x) : __uint_as_float(b.x);
+  r[1] = __uint_as_float(e.residual_bf16 ? b.x & 0xffff0000u : b.y);
+  r[2] = e.residual_bf16 ? bf16_value(b.y) : __uint_as_float(b.z);
+  r[3] = __uint_as_float(e.residual_bf16 ? b.y & 0xffff0000u : b.w);
+}
 // Four outputs n .. n + 3 (n a multiple of four) of row m, those below n_out.
 __device__ __forceinline__ void epilogue_store4(const RowEpilogue &e, const float (&sum)[4], int m, int n, int n_out) {
   if (n >= n_out) return;
   const bool vec = e.vec && n + 4 <= n_out;
-  float r[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
-  if (e.residual && vec) {
-    const long long at = (long long)m * e.residual_stride + n;
-    if (e.residual_bf16) {
-      const uint2 b = *reinterpret_cast<const uint2 *>(reinterpret_cast<const __nv_bfloat16 *>(e.residual) + at);
-      r[0] = bf16_value(b.x); r[1] = __uint_as_float(b.x & 0xffff0000u);
-      r[2] = bf16_value(b.y); r[3] = __uint_as_float(b.y & 0xffff0000u);
-    } else {
-      const float4 b = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(e.residual) + at);
-      r[0] = b.x; r[1] = b.y; r[2] = b.z; r[3] = b.w;
-    }
+  float r[4], f[4];
+  if (vec) {
+    residual4_values(e, residual4_bits(e, m, n), r);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; i++) r[i] = n + i < n_out ? load_residual(e, m, n + i) : 0.f;

@@ -383,7 +383,7 @@ def _gemm_rows(w: DeviceQuantWeight, up: Optional[DeviceQuantWeight], x, bias, b
         res_ptr, res_type = residual.data_ptr(), _row_type(residual, "residual")
     y_stride = n
     if out is None:
-        out = _output(residual if residual is not None and residual.dim() == x.dim() else x, n, out_dtype, stream)
+        out = _output(residual if residual is not None and residual.dim() == 2 == x.dim() else x, n, out_dtype, stream)
     else:
         out_m, y_stride = _rows(out, n, dev, "out")
         if out_m != m:

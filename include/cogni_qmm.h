@@ -405,12 +405,13 @@ int cogni_qmm_gemm_bf16(int type, const void *d_w, const void *d_x_bf16, void *d
  *   residual  NULL, or [m_rows, n_out], f32 or bf16 per residual_type, rows residual_stride (at least n_out)
  *             apart; it may be y itself (same type and stride).  glu: NULL
  *   y         [m_rows, n_out], rows y_stride (at least n_out) elements apart, f32 or bf16 per y_type
- *             (glu: bf16); what lies between the rows is not touched
+ *             (glu: bf16); it overlaps no other input, and what lies between the rows is not touched
  *   k_in a multiple of 256; m_rows at most 4194304
  *   resident  as in cogni_qmm_gemv_resident, for the weights
  * Sums, bias, activation and residual are f32, y is rounded once.  cogni_qmm_gemm_epilogue takes a weight
  * as bf16(dequant(W)), as cogni_qmm_gemm_bf16 does, at any number of rows; cogni_qmm_gemm_glu takes it
- * so or as the f32 dequant(W), whichever its kernel has.
+ * so or as the f32 dequant(W), whichever its kernel has.  A row with infinities or NaN in x gives NaN or
+ * infinities in its own row of y and nowhere else.
  */
 typedef struct cogni_qmm_gemm_args {
   const void *w, *w_up, *x;

@@ -94,7 +94,7 @@ def healthy(engine):
 
 
 # row counts around every boundary of the kernels' tiles, and a few prompt-sized ones
-SHAPES = [(1, 64, 256), (1, 2053, 1024), (2, 300, 768), (7, 129, 512), (8, 1000, 2048), (9, 16, 256), (15, 128, 1280),
+SHAPES = [(5, 1, 256), (2, 3, 768), (40, 7, 512), (90, 2, 256), (1, 64, 256), (1, 2053, 1024), (2, 300, 768), (7, 129, 512), (8, 1000, 2048), (9, 16, 256), (15, 128, 1280),
           (16, 256, 4096), (17, 515, 512), (31, 33, 1024), (33, 130, 256), (63, 513, 768), (64, 384, 2048), (65, 200, 1536),
           (100, 96, 512), (127, 260, 256), (130, 1111, 512), (300, 257, 1024), (700, 300, 512), (1100, 640, 256),
           # enough rows of weights for several parts of K, waves of clusters and every kernel of the gated form
