@@ -37,6 +37,33 @@ int check_rows(const void *p, int type, int64_t stride, int width) {
   return aligned_to(p, type == COGNI_QMM_OUT_BF16 ? 2 : 4) ? COGNI_QMM_OK : COGNI_QMM_ERR_ALIGN;
 }
 
+// Rows as they lie in memory: `width` bytes every `stride` bytes.
+struct Span {
+  const void *p;
+  int64_t stride, width, rows;
+  int type;
+};
+Span span(const void *p, int type, int64_t stride, int64_t rows, int64_t n) {
+  const int64_t size = type == COGNI_QMM_OUT_BF16 ? 2 : 4;
+  return {p, stride * size, n * size, rows, type};
+}
+// Whether a byte belongs to both.  Columns of one buffer may lie side by side; rows of different strides in one stretch
+// of memory count as overlapping.
+bool overlap(const Span &a, const Span &b) {
+  if (!a.p || !b.p) return false;
+  const int64_t pa = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.p)), pb = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.p));
+  if (pa + (a.rows - 1) * a.stride + a.width <= pb || pb + (b.rows - 1) * b.stride + b.width <= pa) return false;
+  if (a.rows == 1 && b.rows == 1) return true;
+  if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) return true;
+  const int64_t stride = a.rows > 1 ? a.stride : b.stride;
+  const int64_t d = ((pb - pa) % stride + stride) % stride;
+  return d < a.width || d + b.width > stride;
+}
+// Element for element the same memory: what a thread has read it may write.
+bool same_rows(const Span &a, const Span &b) {
+  return a.p == b.p && a.type == b.type && a.rows == b.rows && (a.rows == 1 || a.stride == b.stride);
+}
+
 int check_rows_call(const cogni_qmm_gemm_args *a, bool glu, RowsCall &c) {
   if (!a) return COGNI_QMM_ERR_ARG;
   if (!supported(a->type)) return COGNI_QMM_ERR_TYPE;
@@ -54,6 +81,13 @@ int check_rows_call(const cogni_qmm_gemm_args *a, bool glu, RowsCall &c) {
   int st = check_rows(a->y, a->y_type, a->y_stride, a->n_out);
   if (!st && a->residual) st = check_rows(a->residual, a->residual_type, a->residual_stride, a->n_out);
   if (st) return st;
+  const Span y = span(a->y, a->y_type, a->y_stride, a->m_rows, a->n_out);
+  const Span residual = span(a->residual, a->residual_type, a->residual_stride, a->m_rows, a->n_out);
+  if (overlap(y, span(a->x, COGNI_QMM_OUT_BF16, a->x_stride, a->m_rows, a->k_in)) ||
+      overlap(y, span(a->bias, COGNI_QMM_OUT_F32, a->n_out, 1, a->n_out)) ||
+      overlap(y, span(a->bias_up, COGNI_QMM_OUT_F32, a->n_out, 1, a->n_out)) ||
+      (overlap(y, residual) && !same_rows(y, residual)))
+    return COGNI_QMM_ERR_ARG;
   c = {};
   c.type = a->type;
   c.w = a->w; c.w_up = a->w_up;
@@ -462,6 +496,21 @@ int cogni_qmm_norm_residual(const cogni_qmm_norm_args *a, void *stream) {
   if (!st && a->h) st = check_rows(a->h, a->h_type, a->h_stride, a->n);
   if (!st && a->y) st = check_rows(a->y, a->y_type, a->y_stride, a->n);
   if (st) return st;
+  const Span h = span(a->h, a->h_type, a->h_stride, a->m_rows, a->n), y = span(a->y, a->y_type, a->y_stride, a->m_rows, a->n);
+  const Span residual = span(a->residual, a->residual_type, a->residual_stride, a->m_rows, a->n);
+  const Span block = span(a->block, a->block_type, a->block_stride, a->m_rows, a->n);
+  const Span gate = a->gate_stride ? span(a->gate, a->gate_type, a->gate_stride, a->m_rows, a->n)
+                                   : span(a->gate, a->gate_type, a->n, 1, a->n);
+  if (overlap(h, y)) return COGNI_QMM_ERR_ARG;
+  for (const Span &out : {h, y}) {
+    for (const Span &in : {residual, block})
+      if (overlap(out, in) && !same_rows(out, in)) return COGNI_QMM_ERR_ARG;
+    if (overlap(out, gate)) return COGNI_QMM_ERR_ARG;
+    for (const cogni_qmm_norm *s : {&a->post, &a->pre})
+      if (s->weight && (overlap(out, span(s->weight, COGNI_QMM_OUT_F32, a->n, 1, a->n)) ||
+                        overlap(out, span(s->bias, COGNI_QMM_OUT_F32, a->n, 1, a->n))))
+        return COGNI_QMM_ERR_ARG;
+  }
   return launch_norm_residual(*a, static_cast<cudaStream_t>(stream));
 }
 

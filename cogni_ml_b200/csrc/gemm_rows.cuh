@@ -477,7 +477,7 @@ typedef void (*RowsKernel)(CUtensorMap, CUtensorMap, RowsParams);
 
 // Opts into the shared memory, once per device; `once` is the caller's, one per kernel.
 struct RowsOnce {
-  bool configured[64];
+  std::atomic<bool> configured[64];
   int sms[64];
   std::atomic<int> clusters[64][9];  // 1 + how many clusters of that many CTAs run at once
 };

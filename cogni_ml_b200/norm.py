@@ -40,12 +40,12 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
 
     residual, block [M, n], f32 or bf16.  gate: [n] for all rows or [M, n].  Without a block h is the
     residual itself, returned as it is (and not written unless `hidden` is given); without `norm` y is
-    None.  hidden / out: where h and y go; hidden may be residual, out may be block.  h has the
+    None.  hidden / out: where h and y go; each may be residual or block, other overlaps are refused.  h has the
     residual's type unless `hidden` says otherwise, y is out_dtype."""
     n = residual.shape[-1]
     dev = residual.get_device()
-    if dev < 0:
-        raise ValueError("residual must be on a CUDA device")
+    if dev < 0 or not n:
+        raise ValueError("residual must be on a CUDA device and have columns")
     m, res_stride = _rows(residual, n, dev, "residual")
     res_type = _row_type(residual, "residual")
 
@@ -60,7 +60,7 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
         block_ptr, block_stride, block_type = side(block, "block")
         if gate is not None:
             if gate.numel() == n:  # one row for all
-                if not gate.is_contiguous() or gate.get_device() != dev:
+                if gate.shape[-1] != n or not gate.is_contiguous() or gate.get_device() != dev:
                     raise ValueError(f"gate must have {n} contiguous elements, or a row for every row of residual")
                 gate_ptr, gate_type = gate.data_ptr(), _row_type(gate, "gate")
             else:

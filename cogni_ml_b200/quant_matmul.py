@@ -294,7 +294,7 @@ class DeviceQuantWeight:
         """y[m, :] = residual[m, :] + act(W x[m, :] + bias) for any number of rows, x bf16 [M, in_dim].
 
         activation: one of ACTIVATIONS.  bias f32 [out_dim]; residual [M, out_dim] f32 or bf16, which may
-        be `out` itself.  Rows of x, residual and out may be strided (x by a multiple of eight
+        be `out` itself (other overlaps of out and an input are refused).  Rows of x, residual and out may be strided (x by a multiple of eight
         elements).  A weight enters as bf16(dequant(W)), as in `gemm`."""
         return _gemm_rows(self, None, x, bias, None, activation, residual, out_dtype, out, stream)
 

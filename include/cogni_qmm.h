@@ -403,9 +403,10 @@ int cogni_qmm_gemm_bf16(int type, const void *d_w, const void *d_x_bf16, void *d
  *   x         bf16 [m_rows, k_in], rows x_stride elements apart (at least k_in, a multiple of 8), 16-byte aligned
  *   bias, bias_up   NULL, or f32 [n_out]
  *   residual  NULL, or [m_rows, n_out], f32 or bf16 per residual_type, rows residual_stride (at least n_out)
- *             apart; it may be y itself (same type and stride).  glu: NULL
+ *             apart; it may be y itself (same address, type and stride).  glu: NULL
  *   y         [m_rows, n_out], rows y_stride (at least n_out) elements apart, f32 or bf16 per y_type
- *             (glu: bf16); it overlaps no other input, and what lies between the rows is not touched
+ *             (glu: bf16); it overlaps none of x, bias and residual otherwise (COGNI_QMM_ERR_ARG; columns of one buffer
+ *             side by side do not overlap), nor the weights, and what lies between the rows is not touched
  *   k_in a multiple of 256; m_rows at most 4194304
  *   resident  as in cogni_qmm_gemv_resident, for the weights
  * Sums, bias, activation and residual are f32, y is rounded once.  cogni_qmm_gemm_epilogue takes a weight
@@ -439,10 +440,10 @@ int cogni_qmm_gemm_glu(const cogni_qmm_gemm_args *args, void *stream);
  *   block     NULL (h = residual), or [m_rows, n]
  *   post      its norm; post.weight NULL: none.  weight, bias (NULL: none): f32 [n]; eps >= 0
  *   gate      NULL, or [m_rows, n] factors; gate_stride 0: one row for all
- *   h         NULL: not written; may be residual itself (same type and stride)
- *   pre, y    pre.weight NULL: no second norm, y is not written (h is then wanted); y may be block itself
- *             (same type and stride)
- * Strides are in elements, at least n; n at most 32768.  Otherwise the outputs overlap no input.  Sums are
+ *   h         NULL: not written
+ *   pre, y    pre.weight NULL: no second norm, y is not written (h is then wanted)
+ * Strides are in elements, at least n; n at most 32768.  h and y may each be residual or block itself (same
+ * address, type and stride); otherwise they overlap neither each other nor an input (COGNI_QMM_ERR_ARG).  Sums are
  * f32; h and y are rounded once, y from the f32 h.
  */
 typedef struct cogni_qmm_norm {

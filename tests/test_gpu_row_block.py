@@ -409,3 +409,68 @@ def test_calls_on_two_streams_at_once(cuda, oracle, engine):
         got.append((w.dev.gemm_epilogue(x, stream=streams[0]), gemm_glu(w.dev, wu.dev, x2, stream=streams[1])))
     torch.cuda.synchronize()
     assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in got)
+
+
+@pytest.mark.parametrize("qtype", [Q4_K, Q6_K])
+@pytest.mark.parametrize("m", [1, 20, 140])
+def test_columns_of_one_buffer(cuda, oracle, engine, qtype, m):
+    """x, residual and results as columns of one buffer, side by side: not an overlap, and the same bits as apart."""
+    n, k = 136, 512
+    w, x = inputs(cuda, oracle, qtype, m, n, k, seed=71)
+    residual = rows(cuda, m, n, 72, torch.bfloat16)
+    want = w.dev.gemm_epilogue(x, residual=residual, out_dtype=torch.bfloat16)
+    gated = gemm_glu(w.dev, w.dev, x)
+    big = torch.full((m, k + 3 * n + 8), 7.0, device=cuda, dtype=torch.bfloat16)
+    bx, br, by, bg = big[:, :k], big[:, k:k + n], big[:, k + n:k + 2 * n], big[:, k + 2 * n:k + 3 * n]
+    bx.copy_(x)
+    br.copy_(residual)
+    w.dev.gemm_epilogue(bx, residual=br, out=by)
+    gemm_glu(w.dev, w.dev, bx, out=bg)
+    assert torch.equal(by, want) and torch.equal(bg, gated) and torch.equal(bx, x) and (big[:, k + 3 * n:] == 7).all()
+    norm = make_norm(cuda, n, "rms", 73)
+    h, y = norm_residual(br.contiguous(), by.contiguous(), norm=norm)
+    norm_residual(br, by, norm=norm, hidden=br, out=by)
+    assert torch.equal(br, h) and torch.equal(by, y)
+
+
+def test_results_over_inputs_are_refused(cuda, oracle, engine):
+    w = Weight(cuda, oracle, Q4_K, 512, 512, 1)
+    x = rows(cuda, 4, 512, 2, torch.bfloat16)
+    for call in (lambda: w.dev.gemm_epilogue(x, out=x), lambda: gemm_glu(w.dev, w.dev, x, out=x),
+                 lambda: w.dev.gemm_epilogue(x[:3], residual=x[1:], out=x[:3]),
+                 lambda: norm_residual(x, norm=Norm(torch.ones(512, device=cuda)), hidden=x[:], out=x)):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+@pytest.mark.parametrize("qtype", [Q4_K, Q8_0])
+@pytest.mark.parametrize("m", [20, 40, 600])
+def test_rows_past_32_bit_offsets(cuda, oracle, engine, qtype, m):
+    """Rows so far apart that the last ones lie more than 2^32 elements (and bytes) behind the first."""
+    n, k = 264, 512
+    w, x = inputs(cuda, oracle, qtype, m, n, k, seed=81)
+    stride = (1 << 32) // (m - 1) // 8 * 8 + 64
+    far = torch.empty((m - 1) * stride + 1024, device=cuda, dtype=torch.bfloat16)
+    fx, fr = far.as_strided((m, k), (stride, 1), 0), far.as_strided((m, n), (stride, 1), k)
+    fx.copy_(x)
+    residual = rows(cuda, m, n, 82, torch.bfloat16)
+    want = w.dev.gemm_epilogue(x, residual=residual, out_dtype=torch.bfloat16)
+    fr.copy_(residual)
+    assert torch.equal(w.dev.gemm_epilogue(fx, residual=fr, out=fr), want)
+    gated = gemm_glu(w.dev, w.dev, x)
+    assert torch.equal(gemm_glu(w.dev, w.dev, fx, out=fr), gated)
+    norm = make_norm(cuda, n, "layer", 83)
+    h, y = norm_residual(residual, gated, norm=norm)
+    fr.copy_(residual)
+    h2, y2 = norm_residual(fr, gated, norm=norm, hidden=fr)
+    assert torch.equal(h2, h) and torch.equal(y2, y)
+
+
+def test_a_gate_of_one_factor_a_row_is_refused(cuda, engine):
+    with pytest.raises(ValueError, match="gate"):
+        norm_residual(rows(cuda, 8, 8, 1), rows(cuda, 8, 8, 2), gate=rows(cuda, 8, 1, 3))
+
+
+def test_no_columns_are_refused(cuda, engine):
+    with pytest.raises(ValueError, match="columns"):
+        norm_residual(torch.empty(3, 0, device=cuda), norm=Norm(torch.empty(0, device=cuda)))

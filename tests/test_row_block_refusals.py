@@ -90,6 +90,44 @@ def test_structs_have_the_layout_of_the_header(engine, tmp_path):
     assert [line.split(" : ")[0].strip() for line in cr[:cr.index("end")].splitlines()[1:] if " : " in line] == fields[0]
 
 
+X, Y, OTHER = 1 << 20, 1 << 24, 1 << 28  # addresses far apart; nothing there is touched
+APART = dict(x=X, y=Y)
+
+
+@pytest.mark.parametrize("base", [GEMM, GLU], ids=["epilogue", "glu"])
+@pytest.mark.parametrize("changes", [
+    {"y": X}, {"y": X + 2 * 3 * 512 - 4}, {"y": X - 4}, {"y": X, "y_stride": 0}, {"bias": Y}, {"bias": Y + 4 * 63},
+    {"m_rows": 1, "y": X + 1020}, {"x_stride": 1024, "y": X + 1020, "y_stride": 0},
+])
+def test_products_refuse_results_over_their_inputs(engine, base, changes):
+    size = 2 if base is GLU else 4
+    changes = dict(changes)
+    if "y_stride" in changes:  # filled in: the same bytes between rows as x has
+        changes["y_stride"] = changes.get("x_stride", 512) * 2 // size
+    assert gemm(engine, base, **{**APART, **changes}) == ARG
+
+
+@pytest.mark.parametrize("changes", [
+    {"residual": Y + 4, "residual_stride": 64}, {"residual": Y, "residual_stride": 128}, {"residual": Y, "residual_stride": 64, "residual_type": 1},
+    {"residual": Y - 256 * 2, "residual_stride": 64}, {"y_stride": 100, "residual": Y + 252, "residual_stride": 100},
+    {"y_stride": 100, "residual": Y + 200, "residual_stride": 100},
+])
+def test_epilogue_refuses_residuals_half_over_the_result(engine, changes):
+    assert gemm(engine, GEMM, **{**APART, **changes}) == ARG
+
+
+NORM_APART = dict(residual=X, block=2 * X, gate=3 * X, gate_stride=64, h=4 * X, y=5 * X, pre_weight=6 * X)
+
+
+@pytest.mark.parametrize("changes", [
+    {"y": 4 * X}, {"y": 4 * X + 2}, {"h": X + 4}, {"h": X, "h_type": 1}, {"h": X, "h_stride": 65}, {"h": 2 * X},
+    {"y": X}, {"y": 2 * X + 2}, {"y": 3 * X}, {"h": 3 * X}, {"h": 3 * X, "gate_stride": 0}, {"y": 6 * X}, {"h": 6 * X + 252},
+    {"pre_bias": 4 * X}, {"post_weight": 5 * X}, {"post_weight": 7 * X, "post_bias": 4 * X + 256},
+])
+def test_norm_refuses_results_over_their_inputs(engine, changes):
+    assert norm(engine, **{**NORM_APART, **changes}) == ARG
+
+
 # ------------------------------------------------------------------------------- the Python layer
 def weight(engine, device="cpu", n=8, k=256, t=12):
     return engine.DeviceQuantWeight(torch.zeros(n * k // 256 * 144, dtype=torch.uint8, device=device), t, n, k)
