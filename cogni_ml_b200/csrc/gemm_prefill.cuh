@@ -135,6 +135,7 @@ struct GemmParams {
   const uint8_t *w_up;  // kGlu: the second matrix (w is the gate's)
   RowEpilogue epi;      // not kPlain: what happens to a sum on its way out
   float gain;           // kEpilogue: undoes the mean of the accumulation's truncation (mma_gain)
+  int resident;         // the weights were complete before the preceding kernel was launched
 };
 
 // The tile's A rows.  kGlu: row r is row glu_row(r) of the gate (lanes 0-15 of a quarter) or the up
@@ -795,6 +796,16 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams &p, float *part, 
   }
 }
 
+// Programmatic dependent launch of the forms with an epilogue: a grid's barriers, TMEM and (resident) first weights are
+// taken while the grid before it ends.  Its dependents may start once every CTA holds its TMEM, so that none of them
+// takes columns that this grid still waits for.
+template <int MODE> __device__ __forceinline__ void start_dependents() {
+  if constexpr (MODE != kPlain) pdl_launch_dependents();
+}
+template <int MODE> __device__ __forceinline__ void wait_for_inputs() {  // before a thread's first access of x, bias, residual or y
+  if constexpr (MODE != kPlain) pdl_wait_prior_grid();
+}
+
 // ---------------------------------------------------------------------------- the kernel
 template <int TYPE, int BN, bool STAGED, int MODE, bool TWO>
 __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 1)
@@ -863,6 +874,7 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  start_dependents<MODE>();
 
   using R = Roles<isolate_mma_warp(TYPE, STAGED, BN)>;
   if (warp == R::tma_warp) {
@@ -891,9 +903,9 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
             tma_load_2d(win + kRawStage / 2, &tmap_up, Sb<TYPE>::bytes * (sb0 + sbl), raw_n0, full);
         }
       };
-      {
+      if (!p.resident || !STAGED) wait_for_inputs<MODE>();
       if constexpr (STAGED) issue_raw(0);
-      }
+      if (p.resident && STAGED) wait_for_inputs<MODE>();  // resident weights: the first ones beside the preceding kernel
       for (int ks = 0; ks < nks; ks++) {
         const int s = ks % kStages;
         if constexpr (STAGED) {
@@ -1009,6 +1021,7 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
         if (lane < kBatch) mbar_arrive(smem_u32(&bars[(ks + lane) % kStages]));
       }
     } else {
+      if (!p.resident) wait_for_inputs<MODE>();
       fetch_all(0, cur);
       for (int ks = 0; ks < nks; ks++) {
         const int s = ks % kStages;
@@ -1025,6 +1038,7 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
       }
     }
   }
+  wait_for_inputs<MODE>();
   // ---------------------------------------------------------------- epilogue
   const int q = warp & 3;                                  // TMEM lane quarter this warp may read
   const uint32_t taddr = tmem_base + ((uint32_t)(32 * q) << 16);
@@ -1265,6 +1279,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   cluster_sync_all();  // barriers initialised and TMEM allocated in both CTAs
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  start_dependents<MODE>();
 
   using R = Roles<true>;
   if (warp == R::tma_warp) {
@@ -1279,7 +1294,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         tma_load_2d(win, &tmap_w, Sb<TYPE>::bytes * sbl, raw_n0, full);
         if constexpr (MODE == kGlu) tma_load_2d(win + kRawStage / 2, &tmap_up, Sb<TYPE>::bytes * sbl, raw_n0, full);
       };
+      if (!p.resident) wait_for_inputs<MODE>();
       issue_raw(0);
+      if (p.resident) wait_for_inputs<MODE>();
       for (int ks = 0; ks < nks; ks++) {
         const int s = ks % kSB;
         const int sbl = ks >> 2;
@@ -1363,6 +1380,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (lane == 0) mbar_arrive_in_cluster(map_to_cta(smem_u32(&bars[s]), 0));
     }
   }
+  wait_for_inputs<MODE>();
   // ---------------------------------------------------------------- epilogue (own 128 rows)
   const int q = warp & 3;
   const uint32_t taddr = tmem_base + ((uint32_t)(32 * q) << 16);
@@ -1418,6 +1436,12 @@ void split_launch_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute &attr, dim
   attr.val.clusterDim.z = splits;
   cfg.attrs = &attr;
   cfg.numAttrs = splits > 1 ? 1 : 0;
+}
+
+void dependent_launch(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr) {  // attr: room for one more than cfg has
+  attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs++;
 }
 
 // How many clusters of `splits` CTAs run at once (every instance takes a whole SM's shared memory,
@@ -1500,6 +1524,7 @@ GemmParams gemm_params(const RowsCall &c, long long row_bytes, int splits, int k
   p.ks_per_split = ks_per_split;
   p.epi = c.epi;
   p.gain = mma_gain(4 * ks_per_split);
+  p.resident = c.resident;
   return p;
 }
 
@@ -1515,9 +1540,10 @@ int launch(const RowsCall &c, int splits, cudaStream_t s) {
   if (st) return st;
   const GemmParams p = gemm_params(c, row_bytes, splits, ksteps_per_split(c.k_in / kBK, splits));
   cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr;
-  split_launch_config(cfg, attr, dim3((c.n_out + out_rows<MODE>() - 1) / out_rows<MODE>(), (c.m_rows + BN - 1) / BN, splits),
+  cudaLaunchAttribute attr[2];
+  split_launch_config(cfg, attr[0], dim3((c.n_out + out_rows<MODE>() - 1) / out_rows<MODE>(), (c.m_rows + BN - 1) / BN, splits),
                       threads_for(TYPE, STAGED, BN, TWO), smem_for<TYPE, BN, STAGED, TWO>(), splits, s);
+  if (MODE != kPlain) dependent_launch(cfg, attr);
   return (int)cudaLaunchKernelEx(&cfg, gemm_prefill_kernel<TYPE, BN, STAGED, MODE, TWO>, maps[0], maps[1], maps[2], p);
 }
 
@@ -1546,13 +1572,14 @@ int launch_pair(const RowsCall &c, cudaStream_t s) {
   cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (MODE != kPlain) dependent_launch(cfg, attr);
   return (int)cudaLaunchKernelEx(&cfg, gemm_prefill_pair_kernel<TYPE, MODE>, maps[0], maps[1], maps[2], p);
 }
 
