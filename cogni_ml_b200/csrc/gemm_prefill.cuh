@@ -1477,7 +1477,7 @@ void dependent_launch(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr) {  // 
 
 // How many clusters of `splits` CTAs run at once (every instance takes a whole SM's shared memory,
 // so the narrowest one stands for all).
-template <int MODE, bool TWO>
+template <int MODE>
 int split_capacity(int dev, int splits) {
   static std::atomic<int> cached[64][9];  // 1 + the count
   if (dev < 0 || dev >= 64) return 0;
@@ -1486,11 +1486,11 @@ int split_capacity(int dev, int splits) {
   if (v == 0) {
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr;
-    split_launch_config(cfg, attr, dim3(1, 1, splits), threads_for(kQ4_K, true, 128, TWO), smem_for<kQ4_K, 128, true, TWO>(),
+    split_launch_config(cfg, attr, dim3(1, 1, splits), threads_for(kQ4_K, true, 128), smem_for<kQ4_K, 128, true>(),
                         splits, nullptr);
     int n = 0;
-    if (configure<kQ4_K, 128, true, MODE, TWO>(dev) != COGNI_QMM_OK ||
-        cudaOccupancyMaxActiveClusters(&n, gemm_prefill_kernel<kQ4_K, 128, true, MODE, TWO>, &cfg) != cudaSuccess || n < 0) {
+    if (configure<kQ4_K, 128, true, MODE, false>(dev) != COGNI_QMM_OK ||
+        cudaOccupancyMaxActiveClusters(&n, gemm_prefill_kernel<kQ4_K, 128, true, MODE, false>, &cfg) != cudaSuccess || n < 0) {
       cudaGetLastError();  // no split then
       n = 0;
     }
@@ -1663,7 +1663,7 @@ int launch_typed(const RowsCall &c, cudaStream_t s) {
       // Q8_0's direct loads contend where three parts fill the SMs with tiles narrower than the tokens (229 x
       // 2760 x 5376: 128 tokens in three parts 33.7 us, 256 in four on two thirds of the SMs 26.8)
       if (sp == 3 && TYPE == kQ8_0 && widths[i] != 512 && m_rows > widths[i] && g_prefill_force_split != 3) continue;
-      const int at_once = sp == 1 ? sms : split_capacity<MODE, false>(dev, sp);
+      const int at_once = sp == 1 ? sms : split_capacity<MODE>(dev, sp);
       if (at_once == 0) continue;
       const long long tiles = row_tiles * ((m_rows + widths[i] - 1) / widths[i]);
       const int tokens = m_rows < widths[i] ? m_rows : widths[i];
@@ -1676,18 +1676,19 @@ int launch_typed(const RowsCall &c, cudaStream_t s) {
   }
   // Tiles of 128 tokens two CTAs an SM, for the forms with an epilogue: a tile's expansion is a chain of latencies, and
   // two chains of eight warps overlap better than one of sixteen (us: gated Q4_K 12288 x 4096, 128 tokens 66.9 -> 53.4,
-  // Q8_0 8192 x 4096, 100 tokens 38.0 -> 32.4; fitted as above on 33 to 400 tokens, geometric mean over the best plan
-  // 1.06 -> 1.03; tiles of 64 tokens would make it 1.02, and IQ4_NL gains 1.5 %).
+  // Q8_0 8192 x 4096, 100 tokens 38.0 -> 32.4; fitted as above on 33 to 400 tokens, 5139 shapes, 0.7 % over the
+  // fastest plan on average; tiles of 64 tokens would gain 1 %, IQ4_NL 1.5 %).
   constexpr bool kTwo = MODE != kPlain && (TYPE == kQ4_K || TYPE == kQ5_K || TYPE == kQ8_0);
   if constexpr (kTwo) {
     if ((staged || TYPE == kQ8_0) && !g_prefill_force_bn && g_prefill_force_split == 0) {
-      const double fixed = TYPE == kQ8_0 ? 4.90 : 7.15, step = TYPE == kQ8_0 ? 1.196 : 0.742,
-                   column = TYPE == kQ8_0 ? 0.0029 : 0.0070, lone = TYPE == kQ8_0 ? 0.76 : 0.94;
+      const double fixed = TYPE == kQ8_0 ? 2.95 : 7.15, step = TYPE == kQ8_0 ? 1.344 : 0.742,
+                   column = TYPE == kQ8_0 ? 0.0026 : 0.0070, lone = TYPE == kQ8_0 ? 0.87 : 0.94;
       int two_splits = 0;
       for (int sp : {1, 2, 3, 4, 8}) {
         const int per = ksteps_per_split(nks, sp);
         if (sp > 1 && (per < 8 || (sp - 1) * per >= nks)) continue;
-        const int at_once = sp == 1 ? 2 * sms : split_capacity<MODE, true>(dev, sp);
+        // twice as many clusters as of whole SMs: asked about these instances the driver counts one CTA an SM, but two run
+        const int at_once = 2 * (sp == 1 ? sms : split_capacity<MODE>(dev, sp));
         if (at_once == 0) continue;
         const long long tiles = row_tiles * ((m_rows + 127) / 128);
         const double t = fixed + step * per + (sp > 1 ? column * (m_rows < 128 ? m_rows : 128) : 0.0);

@@ -32,6 +32,14 @@ class Norm:
         return _vector(self.weight, n, dev, "weight"), _vector(self.bias, n, dev, "bias"), self.eps, kind
 
 
+def _side(t: torch.Tensor, m: int, n: int, dev: int, name: str):
+    """(address, stride, type) of an [m, n] argument."""
+    rows, stride = _rows(t, n, dev, name)
+    if rows != m:
+        raise ValueError(f"{name} must have a row for every row of residual")
+    return t.data_ptr(), stride, _row_type(t, name)
+
+
 def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, *, post_norm: Optional[Norm] = None,
                   gate: Optional[torch.Tensor] = None, scale: float = 1.0, norm: Optional[Norm] = None,
                   out_dtype=torch.bfloat16, hidden: Optional[torch.Tensor] = None,
@@ -48,32 +56,25 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
         raise ValueError("residual must be on a CUDA device and have columns")
     m, res_stride = _rows(residual, n, dev, "residual")
     res_type = _row_type(residual, "residual")
-
-    def side(t, name):
-        rows, stride = _rows(t, n, dev, name)
-        if rows != m:
-            raise ValueError(f"{name} must have a row for every row of residual")
-        return t.data_ptr(), stride, _row_type(t, name)
-
     block_ptr = block_stride = block_type = gate_ptr = gate_stride = gate_type = 0
     if block is not None:
-        block_ptr, block_stride, block_type = side(block, "block")
+        block_ptr, block_stride, block_type = _side(block, m, n, dev, "block")
         if gate is not None:
             if gate.numel() == n:  # one row for all
                 if gate.shape[-1] != n or not gate.is_contiguous() or gate.get_device() != dev:
                     raise ValueError(f"gate must have {n} contiguous elements, or a row for every row of residual")
                 gate_ptr, gate_type = gate.data_ptr(), _row_type(gate, "gate")
             else:
-                gate_ptr, gate_stride, gate_type = side(gate, "gate")
+                gate_ptr, gate_stride, gate_type = _side(gate, m, n, dev, "gate")
     elif post_norm is not None or gate is not None:
         raise ValueError("post_norm and gate belong to a block")
     elif norm is None:
         raise ValueError("nothing to compute: neither block nor norm")
     h_ptr = h_stride = h_type = 0
     if hidden is not None:
-        h_ptr, h_stride, h_type = side(hidden, "hidden")
+        h_ptr, h_stride, h_type = _side(hidden, m, n, dev, "hidden")
     elif block is not None:
-        hidden = _output(residual, n, residual.dtype, stream)
+        hidden = _output(residual, n, residual.dtype, stream) if stream or res_stride != n else torch.empty_like(residual)
         h_ptr, h_stride, h_type = hidden.data_ptr(), n, res_type
     y_ptr = y_stride = y_type = 0
     if norm is not None:
@@ -81,13 +82,13 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
             out = _output(residual, n, out_dtype, stream)
             y_ptr, y_stride, y_type = out.data_ptr(), n, _ROW_TYPE[out_dtype]
         else:
-            y_ptr, y_stride, y_type = side(out, "out")
+            y_ptr, y_stride, y_type = _side(out, m, n, dev, "out")
     elif out is not None:
         raise ValueError("out is the result of norm")
+    post = _NO_NORM if post_norm is None else post_norm._fields(n, dev)
+    pre = _NO_NORM if norm is None else norm._fields(n, dev)
     args = _NORM_ARGS.pack(residual.data_ptr(), block_ptr, gate_ptr, h_ptr, y_ptr,
-                           res_stride, block_stride, gate_stride, h_stride, y_stride,
-                           *(post_norm._fields(n, dev) if post_norm is not None else _NO_NORM),
-                           *(norm._fields(n, dev) if norm is not None else _NO_NORM),
+                           res_stride, block_stride, gate_stride, h_stride, y_stride, *post, *pre,
                            res_type, block_type, gate_type, h_type, y_type, scale, m, n)
     if m:
         _call(lib.cogni_qmm_norm_residual, "cogni_qmm_norm_residual", args, dev, stream)
