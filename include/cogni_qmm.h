@@ -411,7 +411,7 @@ int cogni_qmm_gemm_bf16(int type, const void *d_w, const void *d_x_bf16, void *d
  *   resident  as in cogni_qmm_gemv_resident, for the weights
  * Sums, bias, activation and residual are f32, y is rounded once.  cogni_qmm_gemm_epilogue takes a weight
  * as bf16(dequant(W)), as cogni_qmm_gemm_bf16 does, at any number of rows; cogni_qmm_gemm_glu takes it
- * so or as the f32 dequant(W), whichever its kernel has.  A row with infinities or NaN in x gives NaN or
+ * so or as the f32 dequant(W), whichever its kernel has (the latter wants |x| below 2^112).  A row with infinities or NaN in x gives NaN or
  * infinities in its own row of y and nowhere else.
  */
 typedef struct cogni_qmm_gemm_args {
