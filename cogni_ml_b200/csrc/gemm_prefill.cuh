@@ -128,13 +128,13 @@ constexpr int kATile = kBM * kBK * 2;  // 16 KB
 struct GemmParams {
   const uint8_t *w;
   void *y;
-  int m_rows, n_out, k_in, out_bf16;
+  int m_rows, n_out, out_bf16;
+  int ks_begin, ks_end;  // the launch's k-steps
   int ks_per_split;  // k-steps per blockIdx.z
   int splits;        // CTAs of a cluster that share a tile along K (1: no cluster)
   long long row_bytes;
   const uint8_t *w_up;  // kGlu: the second matrix (w is the gate's)
   RowEpilogue epi;      // not kPlain: what happens to a sum on its way out
-  float gain;           // kEpilogue: undoes the mean of the accumulation's truncation (mma_gain)
   int resident;         // the weights were complete before the preceding kernel was launched
 };
 
@@ -637,8 +637,7 @@ __device__ __forceinline__ void finish4(const GemmParams &p, const float4 &g, co
   if (MODE == kGlu) {
     glu_store4(p.epi, gv, uv, m, n, p.n_out);
   } else {
-    const float v[4] = {p.gain * g.x, p.gain * g.y, p.gain * g.z, p.gain * g.w};
-    epilogue_store4(p.epi, v, m, n, p.n_out);
+    epilogue_store4(p.epi, gv, m, n, p.n_out);
   }
 }
 // kEpilogue: brings the residual of columns m .. m + cols, rows n .. n + 31 (one warp's share of a
@@ -711,7 +710,7 @@ __device__ __forceinline__ void store_columns(const GemmParams &p, uint32_t tadd
 //
 // finish_columns: the columns of one round (part: [column][128] f32) from token `first` on, by the CTA's warps.  A function
 // of its own: inlined into the loop over the rounds, the constants of all activations stay in registers across it (80 more).
-__device__ __noinline__ void finish_columns(const RowEpilogue e, float gain, const float *part, int first, int live, int n, int n_out) {
+__device__ __noinline__ void finish_columns(const RowEpilogue e, const float *part, int first, int live, int n, int n_out) {
   constexpr int kAhead = 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = (int)blockDim.x >> 5;
   if (e.vec && n + 4 <= n_out) {
@@ -734,7 +733,7 @@ __device__ __noinline__ void finish_columns(const RowEpilogue e, float gain, con
           float f[4];
           residual4_values(e, r[u], f);
 #pragma unroll
-          for (int i = 0; i < 4; i++) f[i] += activate<decltype(act)::value>(fmaf(gain, v[i], bias[i]));
+          for (int i = 0; i < 4; i++) f[i] += activate<decltype(act)::value>(v[i] + bias[i]);
           store_out4(e, first + c + u * nw, n, f);
         }
       }
@@ -743,7 +742,7 @@ __device__ __noinline__ void finish_columns(const RowEpilogue e, float gain, con
 #pragma unroll 1
     for (int c = warp; c < live; c += nw) {
       const float4 s = *reinterpret_cast<const float4 *>(part + c * kBM + 4 * lane);
-      const float v[4] = {gain * s.x, gain * s.y, gain * s.z, gain * s.w};
+      const float v[4] = {s.x, s.y, s.z, s.w};
       epilogue_store4(e, v, first + c, n, n_out);
     }
   }
@@ -767,7 +766,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams &p, float *part, 
       }
     }
     __syncthreads();
-    finish_columns(p.epi, p.gain, part, m0 + r0, live, n0 + 4 * lane, p.n_out);
+    finish_columns(p.epi, part, m0 + r0, live, n0 + 4 * lane, p.n_out);
     __syncthreads();  // the columns have been read
   }
 }
@@ -903,8 +902,8 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
   // host stages only matrices of at least 128 rows); the tile's rows are then further down the box
   const int raw_n0 = STAGED ? min(n0, p.n_out - kRows) : n0;
   // this CTA's k-steps: ks0 .. ks0 + nks - 1 (all of them unless the launch is split along K)
-  const int ks0 = blockIdx.z * p.ks_per_split;
-  const int nks = min(p.ks_per_split, p.k_in / kBK - ks0);
+  const int ks0 = p.ks_begin + blockIdx.z * p.ks_per_split;
+  const int nks = min(p.ks_per_split, p.ks_end - ks0);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; s++) {
@@ -1302,7 +1301,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   constexpr int kRows = out_rows<MODE>();
   const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * kPairBN;
   const int raw_n0 = min(n0, p.n_out - kRows);
-  const int nks = p.k_in / kBK;
+  const int nks = p.ks_end - p.ks_begin;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSA; s++) {
@@ -1336,14 +1335,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   if (warp == R::tma_warp) {
     // ---------------------------------------------------------------- activations and raw weights via TMA
     if (lane == 0) {
-      const int nsb = (nks + 3) >> 2;
+      const int sb0 = p.ks_begin >> 2, nsb = (nks + 3) >> 2;
       auto issue_raw = [&](int sbl) {
         const uint32_t full = smem_u32(&raw_bars[sbl & 1]);
         mbar_arrive_expect_tx(full, kRawStage);
         static_assert(TYPE == kQ4_K || TYPE == kQ5_K, "one box a matrix and superblock column");
         const uint32_t win = smem_u32(raw_win + (sbl & 1) * kRawStage);
-        tma_load_2d(win, &tmap_w, Sb<TYPE>::bytes * sbl, raw_n0, full);
-        if constexpr (MODE == kGlu) tma_load_2d(win + kRawStage / 2, &tmap_up, Sb<TYPE>::bytes * sbl, raw_n0, full);
+        tma_load_2d(win, &tmap_w, Sb<TYPE>::bytes * (sb0 + sbl), raw_n0, full);
+        if constexpr (MODE == kGlu) tma_load_2d(win + kRawStage / 2, &tmap_up, Sb<TYPE>::bytes * (sb0 + sbl), raw_n0, full);
       };
       if (!p.resident) wait_for_inputs<MODE>();
       issue_raw(0);
@@ -1360,7 +1359,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           mbar_wait(smem_u32(&bars[kEmptyB + s * kNSub + h]), ((ks / kSB) & 1) ^ 1);
           const uint32_t full = smem_u32(&bars[kFullB + s * kNSub + h]);
           if (rank == 0) mbar_arrive_expect_tx(full, 2 * kPairBHalf);  // both CTAs' halves of the box
-          tma_load_2d_pair(smem_u32(smem_b + s * kPairBStage + h * kPairBHalf), &tmap_x, ks * kBK,
+          tma_load_2d_pair(smem_u32(smem_b + s * kPairBStage + h * kPairBHalf), &tmap_x, (p.ks_begin + ks) * kBK,
                            m0 + h * 256 + (int)rank * 128, map_to_cta(full, 0));
         }
       }
@@ -1535,26 +1534,19 @@ int encode_maps(const RowsCall &c, int tokens, bool staged, long long row_bytes,
     r = encode_weights<TYPE>(encode, &maps[2], c.w_up, c.n_out, out_rows<MODE>(), row_bytes);
   return (int)r;
 }
-// The tensor core truncates the accumulator at every K = 16 step, which pulls a sum towards zero: by half a unit in
-// the last place of the partial sum, and given its final value y a sum of `steps` terms of any signs stands at
-// y s / steps on average after s of them.  Measured, f32 outputs with K = 2048 .. 32768, weights of four types
-// and activations of mean 0 and 1/2: y comes out (1 - a steps) y, a = 1.30e-8 .. 1.58e-8, about 2^-26.  Taking
-// that mean out halves the error against f64: K = 12288 1.34e-5 -> 6.7e-6 of the norm (a part of a K split
-// counts its own steps).
-float mma_gain(int steps) { return 1.f + (float)steps * 1.4901161e-8f; }
-
-GemmParams gemm_params(const RowsCall &c, long long row_bytes, int splits, int ks_per_split) {
+GemmParams gemm_params(const RowsCall &c, long long row_bytes, int splits) {
   GemmParams p;
   p.w = static_cast<const uint8_t *>(c.w);
   p.w_up = static_cast<const uint8_t *>(c.w_up);
   p.y = c.epi.y;
-  p.m_rows = c.m_rows; p.n_out = c.n_out; p.k_in = c.k_in;
+  p.m_rows = c.m_rows; p.n_out = c.n_out;
   p.out_bf16 = c.epi.y_bf16;
   p.row_bytes = row_bytes;
   p.splits = splits;
-  p.ks_per_split = ks_per_split;
+  p.ks_begin = c.ks_begin;
+  p.ks_end = c.ks_end;
+  p.ks_per_split = ksteps_per_split(c.ks_end - c.ks_begin, splits);
   p.epi = c.epi;
-  p.gain = mma_gain(4 * ks_per_split);
   p.resident = c.resident;
   return p;
 }
@@ -1569,7 +1561,7 @@ int launch(const RowsCall &c, int splits, cudaStream_t s) {
   cudaGetDevice(&dev);
   st = configure<TYPE, BN, STAGED, MODE, TWO>(dev);
   if (st) return st;
-  const GemmParams p = gemm_params(c, row_bytes, splits, ksteps_per_split(c.k_in / kBK, splits));
+  const GemmParams p = gemm_params(c, row_bytes, splits);
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
   split_launch_config(cfg, attr[0], dim3((c.n_out + out_rows<MODE>() - 1) / out_rows<MODE>(), (c.m_rows + BN - 1) / BN, splits),
@@ -1596,7 +1588,7 @@ int launch_pair(const RowsCall &c, cudaStream_t s) {
     if (e != cudaSuccess) return (int)e;
     configured[dev] = true;
   }
-  const GemmParams p = gemm_params(c, row_bytes, 1, c.k_in / kBK);
+  const GemmParams p = gemm_params(c, row_bytes, 1);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * ((c.n_out + 2 * out_rows<MODE>() - 1) / (2 * out_rows<MODE>())),
                      (c.m_rows + kPairBN - 1) / kPairBN, 1);
@@ -1614,9 +1606,26 @@ int launch_pair(const RowsCall &c, cudaStream_t s) {
   return (int)cudaLaunchKernelEx(&cfg, gemm_prefill_pair_kernel<TYPE, MODE>, maps[0], maps[1], maps[2], p);
 }
 
+// Rows that are multiples of 16 bytes (always for Q4_K / Q5_K; Q6_K: in_dim a multiple of 2048) of a matrix with at least
+// one full row tile can be fetched by TMA: the raw superblocks of the tile's rows are then staged through shared memory.
+template <int TYPE, int MODE> bool staged_rows(const RowsCall &c) {
+  const long long row_bytes = (long long)(c.k_in / 256) * Sb<TYPE>::bytes;
+  return TYPE != kQ8_0 && row_bytes % 16 == 0 && c.n_out >= out_rows<MODE>() && g_prefill_stage_raw;
+}
+
+// Token-tile width, parts of K that meet in a cluster, tiles of 128 tokens two CTAs an SM; what that takes, us.
+struct TilePlan {
+  int bn, splits;
+  bool two;
+  double cost;
+};
+
+// the instances of 128 tokens two CTAs an SM (tile_plan)
+template <int TYPE, int MODE> constexpr bool kTwoCtas = MODE != kPlain && (TYPE == kQ4_K || TYPE == kQ5_K || TYPE == kQ8_0);
+
 template <int TYPE, int MODE>
-int launch_typed(const RowsCall &c, cudaStream_t s) {
-  const int m_rows = c.m_rows, n_out = c.n_out, k_in = c.k_in;
+TilePlan tile_plan(const RowsCall &c) {
+  const int m_rows = c.m_rows, n_out = c.n_out;
   // Token-tile width and split along K: wider tiles do less dequant work per flop, narrower ones and
   // splits fill the SMs.  A wave of tiles of 128 / 256 / 512 tokens takes fixed + step x k-steps (a little less
   // where a part of the tile is empty), a split adds the exchange of the partial tiles, per token column; the
@@ -1638,11 +1647,7 @@ int launch_typed(const RowsCall &c, cudaStream_t s) {
     if (dev >= 0 && dev < 64) sms_of[dev] = sms;
   }
   const long long row_tiles = (n_out + out_rows<MODE>() - 1) / out_rows<MODE>();
-  const long long row_bytes = (long long)(k_in / 256) * Sb<TYPE>::bytes;
-  // Rows that are multiples of 16 bytes (always for Q4_K / Q5_K; Q6_K: in_dim a multiple of 2048)
-  // of a matrix with at least one full row tile can be fetched by TMA: the raw superblocks of the
-  // tile's rows are then staged through shared memory
-  const bool staged = TYPE != kQ8_0 && row_bytes % 16 == 0 && n_out >= out_rows<MODE>() && g_prefill_stage_raw;
+  const bool staged = staged_rows<TYPE, MODE>(c);
   struct TileTime { double fixed[3], step[3], column, empty; };
   const TileTime tt = TYPE == kQ6_K ? (staged ? TileTime{{4.40, 5.18, 9.59}, {0.70, 0.79, 0.85}, 0.008, 0.18}
                                               : TileTime{{3.70, 7.22, 7.09}, {1.38, 1.40, 1.57}, 0.011, 0.0})
@@ -1651,10 +1656,13 @@ int launch_typed(const RowsCall &c, cudaStream_t s) {
                                         : TileTime{{5.35, 6.31, 12.94}, {0.49, 0.53, 0.70}, 0.006, 0.0};
   // Few row tiles against many SMs (short prompts, narrow matrices): the CTAs of a cluster take
   // equal parts of K of a tile, two or more superblocks each; the last part takes what is left, at least one.
-  const int nks = k_in / kBK;
+  const int nks = c.ks_end - c.ks_begin;
   const int widths[3] = {128, 256, 512};
-  int bn = 0, splits = 0;
-  double best = 1e30;
+  // the forms with an epilogue: what a plan costs more whose parts of K are too long for an f32 y
+  const auto too_long = [&](int per) {
+    return MODE == kEpilogue && !c.epi.y_bf16 && kBK * per > kMaxF32Part ? 1e7 * per : 0.0;
+  };
+  TilePlan plan = {0, 0, false, 1e30};
   for (int i = 0; i < 3; i++) {
     if (g_prefill_force_bn && g_prefill_force_bn != widths[i]) continue;
     for (int sp : {1, 2, 3, 4, 8}) {
@@ -1669,21 +1677,19 @@ int launch_typed(const RowsCall &c, cudaStream_t s) {
       const int tokens = m_rows < widths[i] ? m_rows : widths[i];
       double t = tt.fixed[i] + tt.step[i] * per * (1.0 - tt.empty * (widths[i] - tokens) / widths[i]);
       if (sp > 1) t += tt.column * tokens;
-      double cost = (double)((tiles + at_once - 1) / at_once) * t;
-      if (g_prefill_force_split >= 2 && sp == g_prefill_force_split) cost -= 1e6;
-      if (cost < best) { best = cost; bn = widths[i]; splits = sp; }
+      double cost = (double)((tiles + at_once - 1) / at_once) * t + too_long(per);
+      if (g_prefill_force_split >= 2 && sp == g_prefill_force_split) cost -= 1e12;
+      if (cost < plan.cost) plan = {widths[i], sp, false, cost};
     }
   }
   // Tiles of 128 tokens two CTAs an SM, for the forms with an epilogue: a tile's expansion is a chain of latencies, and
   // two chains of eight warps overlap better than one of sixteen (us: gated Q4_K 12288 x 4096, 128 tokens 66.9 -> 53.4,
   // Q8_0 8192 x 4096, 100 tokens 38.0 -> 32.4; fitted as above on 33 to 400 tokens, 5139 shapes, 0.7 % over the
   // fastest plan on average; tiles of 64 tokens would gain 1 %, IQ4_NL 1.5 %).
-  constexpr bool kTwo = MODE != kPlain && (TYPE == kQ4_K || TYPE == kQ5_K || TYPE == kQ8_0);
-  if constexpr (kTwo) {
+  if constexpr (kTwoCtas<TYPE, MODE>) {
     if ((staged || TYPE == kQ8_0) && !g_prefill_force_bn && g_prefill_force_split == 0) {
       const double fixed = TYPE == kQ8_0 ? 2.95 : 7.15, step = TYPE == kQ8_0 ? 1.344 : 0.742,
                    column = TYPE == kQ8_0 ? 0.0026 : 0.0070, lone = TYPE == kQ8_0 ? 0.87 : 0.94;
-      int two_splits = 0;
       for (int sp : {1, 2, 3, 4, 8}) {
         const int per = ksteps_per_split(nks, sp);
         if (sp > 1 && (per < 8 || (sp - 1) * per >= nks)) continue;
@@ -1692,14 +1698,22 @@ int launch_typed(const RowsCall &c, cudaStream_t s) {
         if (at_once == 0) continue;
         const long long tiles = row_tiles * ((m_rows + 127) / 128);
         const double t = fixed + step * per + (sp > 1 ? column * (m_rows < 128 ? m_rows : 128) : 0.0);
-        const double cost = tiles * sp > sms ? (double)((tiles + at_once - 1) / at_once) * t : lone * t;  // alone on its SM
-        if (cost < best) { best = cost; two_splits = sp; }
+        const double cost = too_long(per) + (tiles * sp > sms ? (double)((tiles + at_once - 1) / at_once) * t : lone * t);  // alone on its SM
+        if (cost < plan.cost) plan = {128, sp, true, cost};
       }
-      if (two_splits) return launch<TYPE, 128, TYPE != kQ8_0, MODE, true>(c, two_splits, s);
     }
   }
+  return plan;
+}
+
+template <int TYPE, int MODE>
+int launch_plan(const RowsCall &c, const TilePlan &plan, cudaStream_t s) {
+  const int bn = plan.bn, splits = plan.splits;
+  if constexpr (kTwoCtas<TYPE, MODE>) {
+    if (plan.two) return launch<TYPE, 128, TYPE != kQ8_0, MODE, true>(c, splits, s);
+  }
   if constexpr (TYPE != kQ8_0) {
-    if (staged) {
+    if (staged_rows<TYPE, MODE>(c)) {
       if constexpr (TYPE == kQ4_K || TYPE == kQ5_K) {
         if (bn == 512 && splits == 1 && g_prefill_pair)
           return launch_pair<TYPE, MODE>(c, s);
@@ -1712,6 +1726,47 @@ int launch_typed(const RowsCall &c, cudaStream_t s) {
   if (bn == 512) return launch<TYPE, 512, false, MODE>(c, splits, s);
   if (bn == 256) return launch<TYPE, 256, false, MODE>(c, splits, s);
   return launch<TYPE, 128, false, MODE>(c, splits, s);
+}
+
+// What a launch after another costs beside its tiles, us: its start, and y read once more; where the times below lie, Q4_K
+// and Q5_K take clusters and the other types turns.
+constexpr double kTurnCost = 7.0;
+
+template <int TYPE, int MODE>
+int launch_typed(RowsCall c, cudaStream_t s) {
+  const int nks = c.k_in / kBK;
+  c.ks_begin = 0;
+  c.ks_end = nks;
+  const TilePlan plan = tile_plan<TYPE, MODE>(c);
+  if constexpr (MODE == kEpilogue) {
+    // An f32 y whose parts of K have a limit (kMaxF32Part), where no activation follows the sum: the parts may also be
+    // launches one after the other, each adding to what the one before left in y.  That spares the exchange of a cluster and
+    // the tiles that it leaves without a partner.  4096 x 12288, 2048 rows, f32 residual, us, clusters / turns (K whole):
+    // Q4_K 190 / 195 (172), Q6_K 222 / 197 (174), Q8_0 258 / 226 (203), IQ4_NL 213 / 188 (168).
+    const int turns = (nks * kBK + kMaxF32Part - 1) / kMaxF32Part;
+    if (turns > 1 && !c.epi.y_bf16 && c.epi.activation == COGNI_QMM_ACT_NONE && g_prefill_force_split == 0) {
+      const int per = ksteps_per_split(nks, turns);
+      RowsCall part = c;
+      part.ks_end = per;
+      if (turns * (tile_plan<TYPE, MODE>(part).cost + kTurnCost) < plan.cost + kTurnCost) {
+        const float *bias = c.epi.bias;
+        part.epi.bias = nullptr;
+        for (int first = 0; first < nks; first += per) {
+          part.ks_begin = first;
+          part.ks_end = first + per < nks ? first + per : nks;
+          if (part.ks_end == nks) part.epi.bias = bias;
+          const int st = launch_plan<TYPE, MODE>(part, tile_plan<TYPE, MODE>(part), s);
+          if (st) return st;
+          part.epi.residual = c.epi.y;
+          part.epi.residual_stride = c.epi.y_stride;
+          part.epi.residual_bf16 = 0;
+          part.epi.vec = rows_vec4(c.epi.y, c.epi.y_stride, false);
+        }
+        return COGNI_QMM_OK;
+      }
+    }
+  }
+  return launch_plan<TYPE, MODE>(c, plan, s);
 }
 
 template <int MODE>

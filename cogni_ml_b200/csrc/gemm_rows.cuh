@@ -70,7 +70,6 @@ struct RowsParams {
   int m_rows, n_out, nsb, per;  // superblocks of a row, of a part
   int resident;
   int box_rows;  // rows of a TMA box: the tile's of a matrix, or all of them if there are fewer
-  float gain;    // undoes the mean of the accumulation's truncation
   RowEpilogue epi;
 };
 
@@ -295,10 +294,10 @@ __device__ __forceinline__ void finish_rows(const RowsParams &p, const float *pa
     const int row = GLU ? 16 * (o >> 3) + (o & 7) : o;
     const uint32_t at = smem_u32(part + token * (kRows + 4) + row);
     const float4 a = sum_parts(at, parts);
-    const float f[4] = {p.gain * a.x, p.gain * a.y, p.gain * a.z, p.gain * a.w};
+    const float f[4] = {a.x, a.y, a.z, a.w};
     if constexpr (GLU) {
       const float4 b = sum_parts(at + 32, parts);
-      const float u[4] = {p.gain * b.x, p.gain * b.y, p.gain * b.z, p.gain * b.w};
+      const float u[4] = {b.x, b.y, b.z, b.w};
       glu_store4(p.epi, f, u, m0 + token, n0 + o, p.n_out);
     } else {
       epilogue_store4(p.epi, f, m0 + token, n0 + o, p.n_out);
@@ -495,10 +494,6 @@ inline int rows_configure(RowsOnce &once, const void *kernel, int smem, int &sms
   return COGNI_QMM_OK;
 }
 
-// Undoes the mean of the accumulation's truncation over `nsb` superblocks: 2^-26 a step of K = 16 (mma_gain in
-// gemm_prefill.cuh).
-inline float rows_gain(int nsb) { return 1.f + 16.f * (float)nsb * 1.4901161e-8f; }
-
 inline int rows_clusters(RowsOnce &once, RowsKernel kernel, int threads, int smem, int parts) {
   int dev = 0;
   cudaGetDevice(&dev);
@@ -542,12 +537,12 @@ inline int rows_launch(RowsOnce &once, RowsKernel kernel, RowsParams &p, const C
     if (at_once == 0) continue;
     const long long clusters = (long long)blocks * tiles, rest = clusters % at_once * n;  // CTAs of the last wave
     const double load = clusters / at_once * 2.0 + (rest == 0 ? 0.0 : rest <= sms ? 1.3 : 2.0);
-    const double cost = load * (per + 0.75) + (n > 1 ? 0.5 : 0.0);
+    double cost = load * (per + 0.75) + (n > 1 ? 0.5 : 0.0);
+    if (!p.epi.y_bf16 && 256 * per > kMaxF32Part) cost += 1e7 * per;  // the shortest parts if none is short enough
     if (cost < best) { best = cost; parts = n; }
   }
   p.per = (p.nsb + parts - 1) / parts;
   parts = (p.nsb + p.per - 1) / p.per;
-  p.gain = rows_gain(p.per);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks, tiles, parts);
   cfg.blockDim = dim3(threads);
