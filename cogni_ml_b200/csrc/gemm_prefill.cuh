@@ -775,6 +775,9 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams &p, float *part, 
 // k-step: half h0 of the row's 64 (its quarter q2).  What the four k-steps of a superblock share is taken once for all of
 // them: the header, the fifth bits, and the four sub-blocks' scales and minimums as bytes of two words (k-step j has
 // sub-block 2 j + h0), which become floats by permutes.
+//   A warp gives a window back only when what it took from it has been used, here once its weights are stored.  An arrive
+// right behind the loads does not hold until their values are there: the window was filled again before some lanes had them,
+// and with two CTAs an SM one call in ten had rows of a warp expanded from another superblock (gated Q4_K 33 x 4104 x 4352).
 //   raw: the row's block in the first of the two raw windows; tiles: the first weight tile; the barriers by their
 // addresses (full: in the cluster if REMOTE).
 template <int TYPE, bool QUARTER, int kStages, int kTileStride, bool REMOTE>
@@ -814,10 +817,6 @@ __device__ __forceinline__ void produce_k45(const uint8_t *raw, uint32_t raw_ful
         const uint4 v = *reinterpret_cast<const uint4 *>(quants + off + 32 * j + 4 * i);
         qw[i] = v.x; qw[i + 1] = v.y; qw[i + 2] = v.z; qw[i + 3] = v.w;
       }
-      if (j == 3) {  // this warp has read all it needs of the window
-        __syncwarp();
-        if (lane == 0) mbar_arrive(raw_empty + bar);
-      }
       const float sc = __uint_as_float(__byte_perm(sc4, 0x4B000000u, 0x7650 + j)) - 8388608.f;
       const float mn = __uint_as_float(__byte_perm(mn4, 0x4B000000u, 0x7650 + j)) - 8388608.f;
       const float d1 = __fmul_rn(d, sc), m1 = -__fmul_rn(dmin, mn);
@@ -844,6 +843,7 @@ __device__ __forceinline__ void produce_k45(const uint8_t *raw, uint32_t raw_ful
       if (lane == 0) {
         if constexpr (REMOTE) mbar_arrive_in_cluster(full + 8 * s);
         else mbar_arrive(full + 8 * s);
+        if (j == 3) mbar_arrive(raw_empty + bar);
       }
       if (++s == kStages) {
         s = 0;
@@ -1062,10 +1062,6 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
 #pragma unroll
           for (int i = 0; i < kHalves; i++) raws[u][i] = cur[i];
         }
-        if (((ks + kBatch) & 3) == 0) {  // this warp has read all it needs of the window
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&raw_bars[2 + buf]));
-        }
 #pragma unroll
         for (int u = 0; u < kBatch; u++)
           mbar_wait(smem_u32(&bars[kEmptyA + (ks + u) % kStages]), (((ks + u) / kStages) & 1) ^ 1);
@@ -1077,6 +1073,7 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
         fence_async_smem();                                   // generic-proxy writes -> tensor core
         __syncwarp();
         if (lane < kBatch) mbar_arrive(smem_u32(&bars[(ks + lane) % kStages]));
+        if (lane == 0 && ((ks + kBatch) & 3) == 0) mbar_arrive(smem_u32(&raw_bars[2 + buf]));  // see produce_k45
       }
     } else {
       if (!p.resident) wait_for_inputs<MODE>();
