@@ -571,10 +571,8 @@ template <int TYPE, int NT, bool GLU, bool STAGED> int launch_rows_tile(const Ro
 }
 
 template <int TYPE, bool GLU, bool STAGED> int launch_rows_width(const RowsCall &c, cudaStream_t s) {
-  // the narrowest tile that holds all rows (rows_kernel_takes; glu_sums.cuh has up to eight of gated Q4_K / Q5_K)
-  if constexpr (!(GLU && (TYPE == kQ4_K || TYPE == kQ5_K))) {
-    if (c.m_rows <= 8) return launch_rows_tile<TYPE, 1, GLU, STAGED>(c, s);
-  }
+  // the narrowest tile that holds all rows (rows_kernel_takes)
+  if (c.m_rows <= 8) return launch_rows_tile<TYPE, 1, GLU, STAGED>(c, s);
   if (c.m_rows <= 16) return launch_rows_tile<TYPE, 2, GLU, STAGED>(c, s);
   if (c.m_rows <= 24) return launch_rows_tile<TYPE, 3, GLU, STAGED>(c, s);
   if constexpr (TYPE == kQ6_K || TYPE == kQ8_0) {

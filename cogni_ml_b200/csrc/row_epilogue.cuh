@@ -164,12 +164,16 @@ struct RowsCall {
 // is done to a sum, so one that is exact at every step comes out exact.  In bf16 (2^-9) the truncation does not show.
 constexpr int kMaxF32Part = 6144;
 
-// Few rows go to the kernels that expand weights in registers (gemm_rows.cuh, glu_sums.cuh), more to the tensor-core tiles
+// Few rows go to the kernel that expands weights in registers (gemm_rows.cuh), more to the tensor-core tiles
 // (gemm_prefill.cuh), whose expansion into shared memory does not get dearer with the tokens but is slow for Q6_K and Q8_0.
-// Over 6183 drawn shapes, time of the first over that of the best tile, geometric means at 25-32 / 41-48 / 57-64 rows: Q4_K
-// 0.96 / 1.12 / 1.3, Q5_K 0.97 / 1.05 / 1.5, IQ4_NL 0.88 / 1.13 / 1.3, Q8_0 0.57 / 0.74 / 0.87, Q6_K 0.49 / 0.68 / 0.80.
+// Time of the first over that of the best tile, geometric means over drawn shapes:
+//   6183 shapes, at 25-32 / 41-48 / 57-64 rows: Q4_K 0.96 / 1.12 / 1.3, Q5_K 0.97 / 1.05 / 1.5, IQ4_NL 0.88 / 1.13 / 1.3, Q8_0
+//   0.57 / 0.74 / 0.87, Q6_K 0.49 / 0.68 / 0.80;
+//   gated Q4_K and Q5_K, 60 shapes, at 9-16 / 18-24 / 26-32 rows: 0.77 / 0.98 / 1.15, below 2^21 weights a matrix 0.9 throughout.
 inline bool rows_kernel_takes(const RowsCall &c) {
-  return c.m_rows <= (c.type == COGNI_QMM_TYPE_Q6_K || c.type == COGNI_QMM_TYPE_Q8_0 ? 64 : 32);
+  if (c.type == COGNI_QMM_TYPE_Q6_K || c.type == COGNI_QMM_TYPE_Q8_0) return c.m_rows <= 64;
+  const bool gated_k = c.w_up && (c.type == COGNI_QMM_TYPE_Q4_K || c.type == COGNI_QMM_TYPE_Q5_K);
+  return c.m_rows <= (gated_k && (long long)c.n_out * c.k_in >= 1 << 21 ? 24 : 32);
 }
 
 }  // namespace cogni

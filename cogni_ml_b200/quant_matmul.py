@@ -404,7 +404,8 @@ def gemm_glu(gate: DeviceQuantWeight, up: DeviceQuantWeight, x: torch.Tensor, ac
              out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """y[m, :] = act(Wg x[m, :] + bias_gate) * (Wu x[m, :] + bias_up): the gate and up projections of a
     feed-forward block and their product in one launch, for any number of rows.  x bf16 [M, in_dim],
-    y bf16 [M, out_dim] (the down projection's input); rows of x and out may be strided."""
+    y bf16 [M, out_dim] (the down projection's input); rows of x and out may be strided.  A weight enters as
+    bf16(dequant(W)), as in `DeviceQuantWeight.gemm`."""
     if out is not None and out.dtype != torch.bfloat16:
         raise ValueError("out must be bf16")
     return _gemm_rows(gate, up, x, bias_gate, bias_up, activation, None, torch.bfloat16, out, stream)

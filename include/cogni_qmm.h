@@ -409,9 +409,8 @@ int cogni_qmm_gemm_bf16(int type, const void *d_w, const void *d_x_bf16, void *d
  *             side by side do not overlap), nor the weights, and what lies between the rows is not touched
  *   k_in a multiple of 256; m_rows at most 4194304
  *   resident  as in cogni_qmm_gemv_resident, for the weights
- * Sums, bias, activation and residual are f32, y is rounded once.  cogni_qmm_gemm_epilogue takes a weight
- * as bf16(dequant(W)), as cogni_qmm_gemm_bf16 does, at any number of rows; cogni_qmm_gemm_glu takes it
- * so or as the f32 dequant(W), whichever its kernel has (the latter wants |x| below 2^112).  A row with infinities or NaN in x gives NaN or
+ * Sums, bias, activation and residual are f32, y is rounded once.  A weight enters as bf16(dequant(W)), as in
+ * cogni_qmm_gemm_bf16, for every type and number of rows.  A row with infinities or NaN in x gives NaN or
  * infinities in its own row of y and nowhere else.
  */
 typedef struct cogni_qmm_gemm_args {
