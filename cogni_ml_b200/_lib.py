@@ -51,6 +51,7 @@ SIGNATURES = {
     # include/cogni_qmm_diag.h
     "cogni_qmm_set_kernel_choice": (_i, [_i]),
     "cogni_qmm_diag_expire_wait": (_i, [C.c_uint, _vp]),
+    "cogni_qmm_diag_hold": (_i, [C.c_uint, _vp]),
 }
 
 

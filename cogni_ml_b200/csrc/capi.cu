@@ -197,6 +197,8 @@ int cogni_qmm_diag_expire_wait(unsigned limit_us, void *stream) {
   return launch_expire_wait(limit_us, static_cast<cudaStream_t>(stream));
 }
 
+int cogni_qmm_diag_hold(unsigned us, void *stream) { return launch_hold(us, static_cast<cudaStream_t>(stream)); }
+
 unsigned cogni_qmm_wait_timeouts(void) {
   return gemv_imma_timeouts() + gemm_prefill_timeouts() + gemm_epilogue_timeouts() + gemm_glu_timeouts() +
          gemm_rows_epilogue_timeouts() + gemm_rows_glu_timeouts();

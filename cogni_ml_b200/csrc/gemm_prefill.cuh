@@ -771,6 +771,18 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams &p, float *part, 
   }
 }
 
+// Programmatic dependent launch of the forms with an epilogue: a grid's barriers, TMEM and (resident) first weights are
+// taken while the grid before it ends.  Its dependents may start once every CTA holds its TMEM, so that none of them
+// takes columns that this grid still waits for.
+template <int MODE> __device__ __forceinline__ void start_dependents() {
+  if constexpr (MODE != kPlain) pdl_launch_dependents();
+}
+// Before a thread's first access of x, bias, residual or y, and before its first wait for another thread that has to wait
+// here: the limit of a bounded wait (tma_pipe.cuh) does not run while the preceding grid does.
+template <int MODE> __device__ __forceinline__ void wait_for_inputs() {
+  if constexpr (MODE != kPlain) pdl_wait_prior_grid();
+}
+
 // Q4_K / Q5_K, staged: a dequant warp's whole share of a part of K.  A thread has 32 (QUARTER: 16) weights of tile row r in every
 // k-step: half h0 of the row's 64 (its quarter q2).  What the four k-steps of a superblock share is taken once for all of
 // them: the header, the fifth bits, and the four sub-blocks' scales and minimums as bytes of two words (k-step j has
@@ -780,8 +792,8 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams &p, float *part, 
 // and with two CTAs an SM one call in ten had rows of a warp expanded from another superblock (gated Q4_K 33 x 4104 x 4352).
 //   raw: the row's block in the first of the two raw windows; tiles: the first weight tile; the barriers by their
 // addresses (full: in the cluster if REMOTE).
-template <int TYPE, bool QUARTER, int kStages, int kTileStride, bool REMOTE>
-__device__ __forceinline__ void produce_k45(const uint8_t *raw, uint32_t raw_full, uint32_t raw_empty, uint8_t *tiles, uint32_t full,
+template <int TYPE, int MODE, bool QUARTER, int kStages, int kTileStride, bool REMOTE>
+__device__ __forceinline__ void produce_k45(bool resident, const uint8_t *raw, uint32_t raw_full, uint32_t raw_empty, uint8_t *tiles, uint32_t full,
                                             uint32_t empty, int nks, int r, bool valid, int h0, int q2, int lane) {
   constexpr int kWords = QUARTER ? 4 : 8;
   constexpr int kQuants = TYPE == kQ5_K ? 48 : 16;
@@ -792,7 +804,9 @@ __device__ __forceinline__ void produce_k45(const uint8_t *raw, uint32_t raw_ful
   for (int c = 0; c < kWords / 2; c++) at[c] = tiles + r * 128 + (((4 * h0 + (QUARTER ? 2 * q2 : 0) + c) ^ (r & 7)) << 4);
   const uint64_t unbias2 = f2_pack(-8388608.f, -8388608.f);
   uint32_t s = 0, ph = 1;
+  if (!resident) wait_for_inputs<MODE>();
   for (int sbl = 0; 4 * sbl < nks; sbl++) {
+    if (sbl == 1) wait_for_inputs<MODE>();  // the second window is fetched after the inputs are there
     const int off = (sbl & 1) * raw_stage_bytes(TYPE), bar = 8 * (sbl & 1);
     mbar_wait(raw_full + bar, (sbl >> 1) & 1);
     const uint4 hdr = *reinterpret_cast<const uint4 *>(raw + off);
@@ -821,6 +835,7 @@ __device__ __forceinline__ void produce_k45(const uint8_t *raw, uint32_t raw_ful
       const float mn = __uint_as_float(__byte_perm(mn4, 0x4B000000u, 0x7650 + j)) - 8388608.f;
       const float d1 = __fmul_rn(d, sc), m1 = -__fmul_rn(dmin, mn);
       const uint64_t d1_2 = f2_pack(d1, d1), nm1_2 = f2_pack(m1, m1);
+      if (kStages < 4 && j == kStages && sbl == 0) wait_for_inputs<MODE>();  // the first stage that MMAs have to free
       mbar_wait(empty + 8 * s, ph);
 #pragma unroll
       for (int c = 0; c < kWords / 2; c++) {
@@ -851,16 +866,6 @@ __device__ __forceinline__ void produce_k45(const uint8_t *raw, uint32_t raw_ful
       }
     }
   }
-}
-
-// Programmatic dependent launch of the forms with an epilogue: a grid's barriers, TMEM and (resident) first weights are
-// taken while the grid before it ends.  Its dependents may start once every CTA holds its TMEM, so that none of them
-// takes columns that this grid still waits for.
-template <int MODE> __device__ __forceinline__ void start_dependents() {
-  if constexpr (MODE != kPlain) pdl_launch_dependents();
-}
-template <int MODE> __device__ __forceinline__ void wait_for_inputs() {  // before a thread's first access of x, bias, residual or y
-  if constexpr (MODE != kPlain) pdl_wait_prior_grid();
 }
 
 // ---------------------------------------------------------------------------- the kernel
@@ -991,6 +996,7 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
       const uint32_t bar0 = smem_u32(&bars[0]);
       const uint32_t a_lo0 = smem_desc_lo(smem_u32(smem));
       uint32_t s = 0, ph = 0;
+      wait_for_inputs<MODE>();
       for (int ks = 0; ks < nks; ks++) {
         mbar_wait(bar0 + 8 * s, ph);
         const uint32_t a_lo = a_lo0 + s * (kStageBytes >> 4);
@@ -1036,7 +1042,7 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
     };
     if constexpr (STAGED && (TYPE == kQ4_K || TYPE == kQ5_K)) {
       const int rr = min(rn - raw_n0, kRows - 1) + (MODE == kGlu && glu_is_up(r) ? kGluBN : 0);  // its row of the raw boxes
-      produce_k45<TYPE, kQuarter, kStages, kStageBytes, false>(raw_win + rr * Sb<TYPE>::bytes, smem_u32(&raw_bars[0]), smem_u32(&raw_bars[2]),
+      produce_k45<TYPE, MODE, kQuarter, kStages, kStageBytes, false>(p.resident, raw_win + rr * Sb<TYPE>::bytes, smem_u32(&raw_bars[0]), smem_u32(&raw_bars[2]),
                                                                smem, smem_u32(&bars[0]), smem_u32(&bars[kEmptyA]), nks, r, valid, h0, q2, lane);
     } else if constexpr (STAGED) {
       const int sb0 = ks0 >> 2;
@@ -1047,7 +1053,10 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
       // 47.8 -> 44.7, IQ4_NL 44.4 -> 40.6.  Not where only two or three stages fit and the tensor cores
       // would wait for the pair (256 tokens, IQ4_NL 45.7 -> 53.6).
       constexpr int kBatch = BN == 128 ? 2 : 1;
+      constexpr int kFirstWait = kStages < 4 ? kStages / kBatch * kBatch : 4;  // as in produce_k45
+      if (!p.resident) wait_for_inputs<MODE>();
       for (int ks = 0; ks < nks; ks += kBatch) {  // nks is a multiple of four
+        if (ks == kFirstWait) wait_for_inputs<MODE>();
         const int sbl = ks >> 2, buf = sbl & 1;
         if ((ks & 3) == 0) mbar_wait(smem_u32(&raw_bars[buf]), (sbl >> 1) & 1);
         Raw<TYPE> raws[kBatch][kHalves];
@@ -1081,6 +1090,7 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
       for (int ks = 0; ks < nks; ks++) {
         const int s = ks % kStages;
         if (ks + 1 < nks) fetch_all(ks + 1, nxt);             // in flight while this k-step expands
+        if (ks == kStages) wait_for_inputs<MODE>();           // the first stage that MMAs have to free
         mbar_wait(smem_u32(&bars[kEmptyA + s]), ((ks / kStages) & 1) ^ 1);
 #pragma unroll
         for (int i = 0; i < kHalves; i++)
@@ -1370,6 +1380,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const uint32_t bar0 = smem_u32(&bars[0]);
       const uint32_t a_lo0 = smem_desc_lo(smem_u32(smem)), b_lo0 = smem_desc_lo(smem_u32(smem_b));
       uint32_t sa = 0, pa = 0, s = 0, ph = 0;
+      wait_for_inputs<MODE>();
       for (int ks = 0; ks < nks; ks++) {
         mbar_wait(bar0 + 8 * sa, pa);
 #pragma unroll
@@ -1404,7 +1415,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int rn = n0 + (MODE == kGlu ? glu_row(r) : r);   // this row of the matrix
     const bool valid = rn < p.n_out;
     const int rr = min(rn - raw_n0, kRows - 1) + (MODE == kGlu && glu_is_up(r) ? kGluBN : 0);  // its row of the raw boxes
-    produce_k45<TYPE, true, kSA, kATile, true>(raw_win + rr * Sb<TYPE>::bytes, smem_u32(&raw_bars[0]), smem_u32(&raw_bars[2]), smem,
+    produce_k45<TYPE, MODE, true, kSA, kATile, true>(p.resident, raw_win + rr * Sb<TYPE>::bytes, smem_u32(&raw_bars[0]), smem_u32(&raw_bars[2]), smem,
                                                    map_to_cta(smem_u32(&bars[0]), 0), smem_u32(&bars[kEmptyA]), nks, r, valid, h0, q2, lane);
   }
   wait_for_inputs<MODE>();

@@ -2432,6 +2432,12 @@ __global__ void expire_wait_kernel(unsigned long long limit_ns, int *gave_up) {
     if (gave_up) *gave_up = ok ? 0 : 1;
   }
 }
+// Lets the next kernel of the stream start, then runs for a time (at most the two seconds that the host allows).
+__global__ void hold_kernel(unsigned long long ns) {
+  pdl_launch_dependents();
+  const unsigned long long t0 = global_ns();
+  while (global_ns() - t0 < ns) __nanosleep(1000);
+}
 }  // namespace
 
 namespace {
@@ -2463,6 +2469,12 @@ int launch_exchange_unpack(const void *d_words, int64_t n, unsigned epoch, float
 int launch_expire_wait(unsigned limit_us, cudaStream_t s) {
   if (limit_us == 0 || limit_us > 100000) return COGNI_QMM_ERR_ARG;  // at most 0.1 s
   expire_wait_kernel<<<1, 32, 0, s>>>((unsigned long long)limit_us * 1000ull, nullptr);
+  return (int)cudaGetLastError();
+}
+
+int launch_hold(unsigned us, cudaStream_t s) {
+  if (us == 0 || us > 2000000) return COGNI_QMM_ERR_ARG;  // at most two seconds
+  hold_kernel<<<1, 32, 0, s>>>((unsigned long long)us * 1000ull);
   return (int)cudaGetLastError();
 }
 

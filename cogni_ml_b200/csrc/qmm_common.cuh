@@ -159,6 +159,7 @@ unsigned gemm_prefill_timeouts();
 int gemv_imma_reset_timeouts();   // also clears the K-slab tickets of every workspace region
 int gemm_prefill_reset_timeouts();
 int launch_expire_wait(unsigned limit_us, cudaStream_t s);
+int launch_hold(unsigned us, cudaStream_t s);
 int launch_exchange_unpack(const void *d_words, int64_t n, unsigned epoch, float *d_out, cudaStream_t s);
 void gemv_imma_set_debug(int mode);
 void gemv_imma_set_pair(int pair);

@@ -172,6 +172,7 @@ lib LibCogniQMM
   # include/cogni_qmm_diag.h
   fun cogni_qmm_set_kernel_choice(choice : Int32) : Int32
   fun cogni_qmm_diag_expire_wait(limit_us : UInt32, stream : Void*) : Int32
+  fun cogni_qmm_diag_hold(us : UInt32, stream : Void*) : Int32
 end
 
 # Driver-API calls beyond the 28 of driver.cr:1-51 that the engine's host side uses.

@@ -40,6 +40,13 @@ int cogni_qmm_set_kernel_choice(int choice);
  */
 int cogni_qmm_diag_expire_wait(unsigned limit_us, void *stream);
 
+/*
+ * A one-warp kernel that lets its dependents start (programmatic dependent launch) and then runs for
+ * `us` microseconds (1 .. 2000000): what a call of this library finds before it in its stream when the
+ * kernel there takes long.
+ */
+int cogni_qmm_diag_hold(unsigned us, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
