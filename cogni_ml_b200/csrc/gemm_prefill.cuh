@@ -771,6 +771,11 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams &p, float *part, 
   }
 }
 
+// At which of a superblock's four k-steps the copying thread fetches the next superblock's window.  It runs up to `stages`
+// k-steps ahead of the expansion, and the window is free once the expansion has left the superblock before: any earlier it
+// would hold up the activations.
+__host__ __device__ constexpr int raw_turn(int stages) { return stages < 4 ? 2 : 3; }
+
 // Programmatic dependent launch of the forms with an epilogue: a grid's barriers, TMEM and (resident) first weights are
 // taken while the grid before it ends.  Its dependents may start once every CTA holds its TMEM, so that none of them
 // takes columns that this grid still waits for.
@@ -972,9 +977,8 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
         const int s = ks % kStages;
         if constexpr (STAGED) {
           const int sbl = ks >> 2;
-          if ((ks & 3) == 0 && sbl + 1 < nsb) {
-            // the other buffer was last used by superblock sbl - 1: released by the dequant warps
-            // well before the MMAs free this k-step's stage
+          if ((ks & 3) == raw_turn(kStages) && sbl + 1 < nsb) {
+            // the other buffer was last used by superblock sbl - 1
             if (sbl >= 1) mbar_wait(smem_u32(&raw_bars[2 + ((sbl & 1) ^ 1)]), ((sbl - 1) >> 1) & 1);
             issue_raw(sbl + 1);
           }
@@ -1357,7 +1361,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int ks = 0; ks < nks; ks++) {
         const int s = ks % kSB;
         const int sbl = ks >> 2;
-        if ((ks & 3) == 0 && sbl + 1 < nsb) {
+        if ((ks & 3) == raw_turn(kSB) && sbl + 1 < nsb) {
           if (sbl >= 1) mbar_wait(smem_u32(&raw_bars[2 + ((sbl & 1) ^ 1)]), ((sbl - 1) >> 1) & 1);
           issue_raw(sbl + 1);
         }
