@@ -333,6 +333,9 @@ module ML::CUDA
     # y[m, :] = act(gate x[m, :]) * (up x[m, :]) as bf16; self is the gate.
     def gemm_glu(up : DeviceQuantWeight, x_bf16 : DeviceBuffer, y_bf16 : DeviceBuffer, m_rows : Int32,
                  activation : Int32 = LibCogniQMM::ACT_SILU, stream : Void* = ML::CUDA.current_stream) : Nil
+      unless up.type == @type && up.out_dim == @out_dim && up.in_dim == @in_dim
+        raise ArgumentError.new("gate and up must have the same type and shape")
+      end
       args = rows_args(x_bf16, y_bf16, m_rows, true, activation)
       args.w_up = up.buffer.ptr
       ML::CUDA.qmm_check! LibCogniQMM.cogni_qmm_gemm_glu(pointerof(args), stream), "cogni_qmm_gemm_glu"
