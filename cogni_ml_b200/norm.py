@@ -9,7 +9,7 @@ from typing import Optional
 import torch
 
 from ._lib import lib
-from .quant_matmul import _ROW_TYPE, _call, _output, _row_type, _rows, _vector
+from .quant_matmul import _ROW_TYPE, _call, _output, _record, _row_type, _rows, _vector
 
 _KINDS = {"rms": 0, "layer": 1}
 _NORM_ARGS = struct.Struct("5Q5q2Qfi2Qfi5if2i")  # cogni_qmm_norm_args
@@ -92,4 +92,9 @@ def norm_residual(residual: torch.Tensor, block: Optional[torch.Tensor] = None, 
                            res_type, block_type, gate_type, h_type, y_type, scale, m, n)
     if m:
         _call(lib.cogni_qmm_norm_residual, "cogni_qmm_norm_residual", args, dev, stream)
+        if stream:
+            _record(stream, residual, block, gate, hidden, out)
+            for side in (post_norm, norm):
+                if side is not None:
+                    _record(stream, side.weight, side.bias)
     return hidden if hidden is not None else residual, out

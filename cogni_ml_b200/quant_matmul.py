@@ -295,7 +295,8 @@ class DeviceQuantWeight:
 
         activation: one of ACTIVATIONS.  bias f32 [out_dim]; residual [M, out_dim] f32 or bf16, which may
         be `out` itself (other overlaps of out and an input are refused).  Rows of x, residual and out may be strided (x by a multiple of eight
-        elements).  A weight enters as bf16(dequant(W)), as in `gemm`."""
+        elements).  A weight enters as bf16(dequant(W)), as in `gemm`.  With `stream` the caller orders the inputs before
+        the call there and the result's readers after it; their memory is kept until that stream is done with it."""
         return _gemm_rows(self, None, x, bias, None, activation, residual, out_dtype, out, stream)
 
 
@@ -351,13 +352,26 @@ def _output(like: torch.Tensor, width: int, dtype, stream) -> torch.Tensor:
     """A new tensor with the rows of `like`, `width` columns and the given type."""
     if dtype not in _ROW_TYPE:
         raise ValueError(f"outputs are f32 or bf16, not {dtype}")
+    if stream:
+        # from the pool of the stream that writes it: a block of the current stream's may still be in use by work queued
+        # there.  The caller reads it on the current one.
+        current = torch.cuda.current_stream(like.device)
+        with torch.cuda.stream(stream):
+            out = _output(like, width, dtype, None)
+        out.record_stream(current)
+        return out
     if like.shape[-1] == width and like.is_contiguous():
         out = torch.empty_like(like) if like.dtype is dtype else torch.empty_like(like, dtype=dtype)
     else:
         out = like.new_empty(like.shape[:-1] + (width,), dtype=dtype)
-    if stream:  # allocated on the current stream, written on another
-        out.record_stream(stream)
     return out
+
+
+def _record(stream, *tensors: Optional[torch.Tensor]) -> None:
+    """Keeps the memory of what a call on another stream reads and writes until that stream is done with it."""
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
 
 
 def _gemm_rows(w: DeviceQuantWeight, up: Optional[DeviceQuantWeight], x, bias, bias_up, activation, residual,
@@ -396,6 +410,8 @@ def _gemm_rows(w: DeviceQuantWeight, up: Optional[DeviceQuantWeight], x, bias, b
             _call(lib.cogni_qmm_gemm_epilogue, "cogni_qmm_gemm_epilogue", args, dev, stream)
         else:
             _call(lib.cogni_qmm_gemm_glu, "cogni_qmm_gemm_glu", args, dev, stream)
+        if stream:
+            _record(stream, x, bias, bias_up, residual, out)
     return out
 
 
