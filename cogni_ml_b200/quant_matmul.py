@@ -78,6 +78,26 @@ def _stream_ptr(stream: Optional[torch.cuda.Stream]) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
+def _new(make, stream, device, *shape, dtype):
+    """make(*shape), torch.empty or torch.zeros, for a call on `stream` (None: the current one): from the pool and in the order
+    of the stream that uses it, since a block of the current stream's may still be in use by work queued there."""
+    if not stream:
+        return make(*shape, dtype=dtype, device=device)
+    current = torch.cuda.current_stream(device)
+    with torch.cuda.stream(stream):
+        out = make(*shape, dtype=dtype, device=device)
+    out.record_stream(current)  # the caller reads it there
+    return out
+
+
+def _record(stream, *tensors: Optional[torch.Tensor]) -> None:
+    """Keeps the memory of what a call on another stream reads and writes until that stream is done with it."""
+    if stream:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
 def _require_cuda() -> None:
     if not torch.cuda.is_available():
         raise RuntimeError("cogni_ml_b200 needs a CUDA device (sm_100a); there is no CPU fallback")
@@ -144,7 +164,7 @@ class DeviceQuantWeight:
 
     def dequantize(self, stream=None) -> torch.Tensor:
         """f32 [out_dim, in_dim], bit-identical to Dequant.dequantize on the CPU."""
-        out = torch.empty(self.out_dim, self.in_dim, dtype=torch.float32, device=self.raw.device)
+        out = _new(torch.empty, stream, self.raw.device, self.out_dim, self.in_dim, dtype=torch.float32)
         check(lib.cogni_qmm_dequantize(self.type, self.raw.data_ptr(), self.out_dim * self.in_dim,
                                        out.data_ptr(), _stream_ptr(stream)), "cogni_qmm_dequantize")
         return out
@@ -157,7 +177,7 @@ class DeviceQuantWeight:
             raise ValueError("x must be contiguous f32 [batch, in_dim]")
         batch = x.numel() // self.in_dim
         if out is None:
-            out = torch.empty(batch, self.out_dim, dtype=torch.float32, device=x.device)
+            out = _new(torch.empty, stream, x.device, batch, self.out_dim, dtype=torch.float32)
         if bias is not None and residual is not None:
             raise ValueError("pass bias or residual, not both")
         addend, stride = (bias, 0) if bias is not None else (residual, self.out_dim)
@@ -166,6 +186,7 @@ class DeviceQuantWeight:
                  addend.data_ptr() if addend is not None else None, stride,
                  out.data_ptr(), self.in_dim, self.out_dim, batch, _stream_ptr(stream)),
               "cogni_qmm_gemv")
+        _record(stream, x, addend, out)
         return out
 
     def gemv_top2(self, x: torch.Tensor, stream=None, want_keys: bool = False):
@@ -178,16 +199,17 @@ class DeviceQuantWeight:
         need = lib.cogni_qmm_gemv_top2_scratch_bytes(self.out_dim, batch)
         scratch = getattr(self, "_top2_scratch", None)
         if scratch is None or scratch.numel() < need:
-            scratch = self._top2_scratch = torch.zeros(need, dtype=torch.uint8, device=self.raw.device)
-        idx = torch.empty(batch, 2, dtype=torch.int32, device=x.device)
-        val = torch.empty(batch, 2, dtype=torch.float32, device=x.device)
-        key = torch.empty(batch, 2, dtype=torch.int64, device=x.device) if want_keys else None
+            scratch = self._top2_scratch = _new(torch.zeros, stream, self.raw.device, need, dtype=torch.uint8)
+        idx = _new(torch.empty, stream, x.device, batch, 2, dtype=torch.int32)
+        val = _new(torch.empty, stream, x.device, batch, 2, dtype=torch.float32)
+        key = _new(torch.empty, stream, x.device, batch, 2, dtype=torch.int64) if want_keys else None
         check(lib.cogni_qmm_gemv_top2(self.type, self.raw.data_ptr(), x.data_ptr(), self.in_dim,
                                       self.out_dim, batch, self.row_begin, scratch.data_ptr(),
                                       scratch.numel(), idx.data_ptr(), val.data_ptr(),
                                       key.data_ptr() if key is not None else None,
                                       1 if self.resident else 0, _stream_ptr(stream)),
               "cogni_qmm_gemv_top2")
+        _record(stream, x, scratch)
         return (idx, val, key) if want_keys else (idx, val)
 
     def embedding_lookup(self, token_ids: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -199,13 +221,16 @@ class DeviceQuantWeight:
             raise ValueError("token_ids must be a contiguous int32 tensor")
         n = token_ids.numel()
         if out is None:
-            out = torch.empty(n, self.in_dim, dtype=torch.float32, device=token_ids.device)
-        status = torch.zeros(1, dtype=torch.int32, device=token_ids.device) if check_range else None
+            out = _new(torch.empty, stream, token_ids.device, n, self.in_dim, dtype=torch.float32)
+        status = _new(torch.zeros, stream, token_ids.device, 1, dtype=torch.int32) if check_range else None
         check(lib.cogni_qmm_embedding_lookup(self.type, self.raw.data_ptr(), self.out_dim, self.in_dim,
                                              token_ids.data_ptr(), n, out.data_ptr(),
                                              status.data_ptr() if status is not None else None,
                                              _stream_ptr(stream)), "cogni_qmm_embedding_lookup")
+        _record(stream, token_ids, out)
         if status is not None:
+            if stream:
+                stream.synchronize()
             bad = int(status.item())
             if bad:
                 raise IndexError(f"embedding: token_id {int(token_ids.view(-1)[bad - 1])} out of range")
@@ -220,25 +245,25 @@ class DeviceQuantWeight:
                 raise ValueError("gate and up must be contiguous f32 [batch, in_dim]")
         batch = gate.numel() // self.in_dim
         if out is None:
-            out = torch.empty(batch, self.out_dim, dtype=torch.float32, device=gate.device)
+            out = _new(torch.empty, stream, gate.device, batch, self.out_dim, dtype=torch.float32)
         # shapes the fused kernel does not take (and the diagnostic row-per-warp mode) need room
         # for the product; the buffer is kept with the weight
         scratch = getattr(self, "_swiglu_scratch", None)
         if scratch is None or scratch.numel() < gate.numel() or scratch.device != gate.device:
-            scratch = self._swiglu_scratch = torch.empty(gate.numel(), dtype=torch.float32,
-                                                         device=gate.device)
+            scratch = self._swiglu_scratch = _new(torch.empty, stream, gate.device, gate.numel(), dtype=torch.float32)
         check(lib.cogni_qmm_gemv_swiglu(self.type, self.raw.data_ptr(), gate.data_ptr(), up.data_ptr(),
                                         residual.data_ptr() if residual is not None else None,
                                         self.out_dim if residual is not None else 0, out.data_ptr(),
                                         scratch.data_ptr(),
                                         self.in_dim, self.out_dim, batch, 1 if self.resident else 0,
                                         _stream_ptr(stream)), "cogni_qmm_gemv_swiglu")
+        _record(stream, gate, up, residual, out, scratch)
         return out
 
-    def top1_scratch(self, batch: int) -> torch.Tensor:
+    def top1_scratch(self, batch: int, stream=None) -> torch.Tensor:
         need = lib.cogni_qmm_gemv_top1_scratch_bytes(self.out_dim, batch)
         if self._top1_scratch is None or self._top1_scratch.numel() < need:
-            self._top1_scratch = torch.zeros(need, dtype=torch.uint8, device=self.raw.device)
+            self._top1_scratch = _new(torch.zeros, stream, self.raw.device, need, dtype=torch.uint8)
         return self._top1_scratch
 
     def gemv_top1(self, x: torch.Tensor, stream=None, want_keys: bool = False,
@@ -250,12 +275,13 @@ class DeviceQuantWeight:
         if x.dtype != torch.float32 or not x.is_contiguous() or x.shape[-1] != self.in_dim:
             raise ValueError("x must be contiguous f32 [batch, in_dim]")
         batch = x.numel() // self.in_dim
-        scratch = self.top1_scratch(batch)
-        idx = torch.empty(batch, dtype=torch.int32, device=x.device)
-        val = torch.empty(batch, dtype=torch.float32, device=x.device)
-        key = torch.empty(batch, dtype=torch.int64, device=x.device) if want_keys else None
+        scratch = self.top1_scratch(batch, stream)
+        idx = _new(torch.empty, stream, x.device, batch, dtype=torch.int32)
+        val = _new(torch.empty, stream, x.device, batch, dtype=torch.float32)
+        key = _new(torch.empty, stream, x.device, batch, dtype=torch.int64) if want_keys else None
+        _record(stream, x, scratch, norm_weight)
         if norm_weight is not None:
-            xs = torch.empty_like(x)   # for shapes the fused kernel does not take
+            xs = _new(torch.empty, stream, x.device, *x.shape, dtype=x.dtype)   # for shapes the fused kernel does not take
             check(lib.cogni_qmm_gemv_top1_rmsnorm(self.type, self.raw.data_ptr(), x.data_ptr(),
                                                   norm_weight.data_ptr(), float(eps), self.in_dim,
                                                   self.out_dim, batch, self.row_begin,
@@ -280,11 +306,12 @@ class DeviceQuantWeight:
             raise ValueError("x must be contiguous bf16 [M, in_dim]")
         m = x_bf16.numel() // self.in_dim
         if out is None:
-            out = torch.empty(m, self.out_dim, dtype=out_dtype, device=x_bf16.device)
+            out = _new(torch.empty, stream, x_bf16.device, m, self.out_dim, dtype=out_dtype)
         code = {torch.float32: 0, torch.bfloat16: 1}[out.dtype]
         check(lib.cogni_qmm_gemm_bf16(self.type, self.raw.data_ptr(), x_bf16.data_ptr(),
                                       out.data_ptr(), code, m, self.out_dim, self.in_dim,
                                       _stream_ptr(stream)), "cogni_qmm_gemm_bf16")
+        _record(stream, x_bf16, out)
         return out
 
 
@@ -367,13 +394,6 @@ def _output(like: torch.Tensor, width: int, dtype, stream) -> torch.Tensor:
     return out
 
 
-def _record(stream, *tensors: Optional[torch.Tensor]) -> None:
-    """Keeps the memory of what a call on another stream reads and writes until that stream is done with it."""
-    for t in tensors:
-        if t is not None:
-            t.record_stream(stream)
-
-
 def _gemm_rows(w: DeviceQuantWeight, up: Optional[DeviceQuantWeight], x, bias, bias_up, activation, residual,
                out_dtype, out, stream) -> torch.Tensor:
     n, k, raw = w.out_dim, w.in_dim, w.raw
@@ -410,8 +430,7 @@ def _gemm_rows(w: DeviceQuantWeight, up: Optional[DeviceQuantWeight], x, bias, b
             _call(lib.cogni_qmm_gemm_epilogue, "cogni_qmm_gemm_epilogue", args, dev, stream)
         else:
             _call(lib.cogni_qmm_gemm_glu, "cogni_qmm_gemm_glu", args, dev, stream)
-        if stream:
-            _record(stream, x, bias, bias_up, residual, out)
+        _record(stream, x, bias, bias_up, residual, out)
     return out
 
 
@@ -488,8 +507,11 @@ def gemv_many(weights, x: torch.Tensor, outs=None, stream=None, norm_weight=None
     launch."""
     batch = x.numel() // weights[0].in_dim
     if outs is None:
-        outs = [torch.empty(batch, w.out_dim, dtype=torch.float32, device=x.device) for w in weights]
-    return GemvMany(weights, x, outs, norm_weight=norm_weight, eps=eps).run(stream)
+        outs = [_new(torch.empty, stream, x.device, batch, w.out_dim, dtype=torch.float32) for w in weights]
+    with torch.cuda.stream(stream or None):  # its scratch, as in _new
+        GemvMany(weights, x, outs, norm_weight=norm_weight, eps=eps).run(stream)
+    _record(stream, x, norm_weight, *outs)
+    return outs
 
 
 def unpack_top1_keys(keys: torch.Tensor):
