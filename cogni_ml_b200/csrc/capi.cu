@@ -168,6 +168,10 @@ int cogni_qmm_set_kernel_choice(int choice) {
     gemm_prefill_set_pair(choice == 57);
     return COGNI_QMM_OK;
   }
+  if (choice == 71 || choice == 72) {  // the forms with an epilogue, 128-token tiles two CTAs an SM: automatic (71, default) / always
+    gemm_prefill_set_two(choice == 72);
+    return COGNI_QMM_OK;
+  }
   if (choice >= 52 && choice <= 54) {  // prefill split along K: automatic / never / two parts wherever allowed
     gemm_prefill_set_split(choice - 52);
     return COGNI_QMM_OK;

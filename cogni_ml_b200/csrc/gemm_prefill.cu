@@ -7,6 +7,7 @@ int g_prefill_force_bn = 0;
 int g_prefill_stage_raw = 1;
 int g_prefill_force_split = 0;
 int g_prefill_pair = 1;
+int g_prefill_two = 0;
 
 int launch_gemm_prefill(int type, const void *d_w, const void *d_x_bf16, void *d_y, int out_type,
                         int m_rows, int n_out, int k_in, cudaStream_t s) {
@@ -26,6 +27,7 @@ void gemm_prefill_set_tile(int bn) { g_prefill_force_bn = bn; }
 void gemm_prefill_set_split(int mode) { g_prefill_force_split = mode; }
 void gemm_prefill_set_stage_raw(int on) { g_prefill_stage_raw = on; }
 void gemm_prefill_set_pair(int on) { g_prefill_pair = on; }
+void gemm_prefill_set_two(int on) { g_prefill_two = on; }
 
 unsigned gemm_prefill_timeouts() { return form_timeouts(); }
 int gemm_prefill_reset_timeouts() { return form_reset_timeouts(); }

@@ -53,6 +53,7 @@ extern int g_prefill_force_bn;     // 0 = automatic, else the token-tile width t
 extern int g_prefill_stage_raw;    // 0 = dequant threads read global memory directly
 extern int g_prefill_force_split;  // 0 = automatic, 1 = never split along K, else that many parts where allowed
 extern int g_prefill_pair;         // 0 = the one-CTA kernel for 512-token tiles too
+extern int g_prefill_two;          // 1 = 128-token tiles two CTAs an SM wherever there is such an instance
 
 namespace {
 
@@ -1699,18 +1700,20 @@ TilePlan tile_plan(const RowsCall &c) {
   // Q8_0 8192 x 4096, 100 tokens 38.0 -> 32.4; fitted as above on 33 to 400 tokens, 5139 shapes, 0.7 % over the
   // fastest plan on average; tiles of 64 tokens would gain 1 %, IQ4_NL 1.5 %).
   if constexpr (kTwoCtas<TYPE, MODE>) {
-    if ((staged || TYPE == kQ8_0) && !g_prefill_force_bn && g_prefill_force_split == 0) {
+    if ((staged || TYPE == kQ8_0) && (g_prefill_two || (!g_prefill_force_bn && g_prefill_force_split == 0))) {
       const double fixed = TYPE == kQ8_0 ? 2.95 : 7.15, step = TYPE == kQ8_0 ? 1.344 : 0.742,
                    column = TYPE == kQ8_0 ? 0.0026 : 0.0070, lone = TYPE == kQ8_0 ? 0.87 : 0.94;
       for (int sp : {1, 2, 3, 4, 8}) {
         const int per = ksteps_per_split(nks, sp);
-        if (sp > 1 && (per < 8 || (sp - 1) * per >= nks)) continue;
-        // twice as many clusters as of whole SMs: asked about these instances the driver counts one CTA an SM, but two run
+        if (sp > 1 && (per < 8 || (sp - 1) * per >= nks || g_prefill_force_split == 1)) continue;
+        // twice as many clusters as of whole SMs (split_capacity asks the driver about an instance that fills an SM): asked about
+        // the instances here it counts one CTA an SM too, but two run
         const int at_once = 2 * (sp == 1 ? sms : split_capacity<MODE>(dev, sp));
         if (at_once == 0) continue;
         const long long tiles = row_tiles * ((m_rows + 127) / 128);
         const double t = fixed + step * per + (sp > 1 ? column * (m_rows < 128 ? m_rows : 128) : 0.0);
-        const double cost = too_long(per) + (tiles * sp > sms ? (double)((tiles + at_once - 1) / at_once) * t : lone * t);  // alone on its SM
+        double cost = too_long(per) + (tiles * sp > sms ? (double)((tiles + at_once - 1) / at_once) * t : lone * t);  // alone on its SM
+        if (g_prefill_two) cost -= g_prefill_force_split >= 2 && sp == g_prefill_force_split ? 3e12 : 2e12;
         if (cost < plan.cost) plan = {128, sp, true, cost};
       }
     }

@@ -169,6 +169,7 @@ void gemm_prefill_set_tile(int bn);
 void gemm_prefill_set_split(int mode);
 void gemm_prefill_set_stage_raw(int on);
 void gemm_prefill_set_pair(int on);
+void gemm_prefill_set_two(int on);
 
 // Kernel selection (dispatch.cu): picks the tiled kernel when the shape allows it, else the
 // general row-per-warp kernel.

@@ -37,8 +37,8 @@ template <class F> __device__ __forceinline__ void with_activation(int act, F &&
   }
 }
 
-// In f32.  exp(-v) overflows to infinity for v < -88, where v / infinity = -0 and 1 / infinity = 0 are
-// the limits.  The tanh form is v * sigmoid(2 u), the same function without the cancellation of
+// In f32.  The quotients are 0 where exp(-v) is above 2^126 (v < -87.3, __fdividef), which is within 2^-126 |v| of the value.
+// __expf is off by 2 + 1.17 |v| units of 2^-23, so sigmoid and silu by 1e-5 of their value at v = -80 where that is 1e-35.  The tanh form is v * sigmoid(2 u), the same function without the cancellation of
 // 1 + tanh(u) at negative u.
 template <int ACT> __device__ __forceinline__ float activate(float v) {
   if (ACT == COGNI_QMM_ACT_RELU) return v < 0.f ? 0.f : v;  // NaN stays NaN

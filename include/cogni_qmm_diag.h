@@ -24,6 +24,8 @@ extern "C" {
  *   55-56     prefill raw superblocks staged by TMA (default) / read directly by the dequant threads
  *   57-58     prefill 512-token tiles of Q4_K / Q5_K on CTA pairs (default) / on single CTAs
  *   59, 69, 70  prefill split along K: four / eight / three parts wherever allowed (52 returns to automatic)
+ *   71-72     prefill forms with an epilogue, 128-token tiles two CTAs an SM: automatic / wherever there
+ *             is such a kernel (Q4_K, Q5_K, Q8_0), with the split of 52-54, 59, 69, 70
  *   60-68     K slabs of the tiled GEMV (several CTAs share a row tile, partial sums meet in a
  *             workspace): 60 = off (default), 61-68 = 1 .. 8 slabs wherever a plan allows it
  * Returns COGNI_QMM_ERR_ARG for any other value.  (A library built with -DCOGNI_QMM_DIAG_TIMING
