@@ -12,7 +12,7 @@
 // four consecutive weights of lane t, and the B operand is read from the activations accordingly.
 //   * A CTA is eight warps (128 weight rows) and a part of K; the parts of a row block form a cluster and
 //     meet in distributed shared memory (cluster_sum.cuh), so no workspace, no atomics, the same bits every
-//     time.  K is cut until the CTAs fill the SMs twice.
+//     time.  K is cut where waves x superblocks come out least (rows_launch).
 //   * A superblock column of the CTA's rows (one TMA box a matrix) and the tokens' 256 activations (16-byte
 //     cp.async) are one stage of a ring; all loads of a short part are in flight at once.  Q6_K rows that
 //     are not multiples of 16 bytes (k_in not a multiple of 2048) cannot be described to TMA: their
@@ -406,7 +406,11 @@ __global__ void __launch_bounds__(kRowThreads, 2)
 #pragma unroll 1
   for (int i = 0; i < nsb; i++) {
     cp_async_wait<kStages - 2>();
-    if constexpr (STAGED) ok &= mbar_wait(bars + 8 * (i % kStages), (i / kStages) & 1);
+    if constexpr (STAGED) {
+      ok &= mbar_wait(bars + 8 * (i % kStages), (i / kStages) & 1);
+      // the barrier orders the reads of stage i - 1 against threads, this against the TMA copy that fills it again (0.4 %)
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     __syncthreads();  // stage i has landed for every warp, stage i - 1 is free
     if (i + kStages - 1 < nsb) {
       issue_weights(i + kStages - 1);
