@@ -317,6 +317,11 @@ template <int NT, int kRows> __device__ __forceinline__ void leave_tile(const fl
   }
 }
 
+// Whether the tensor cores' sums, truncated at every step (kMaxF32Part), are taken a superblock at a time and added rounded to
+// nearest: Q6_K 4096 x 12288, one row, 1.6e-6 -> 2.4e-7 of the norm, at the same time.  The gated form's bf16 result does not
+// need it, and more than 32 tokens have no registers for it (3.4e-6).
+template <int NT, bool GLU> constexpr bool kBySuperblock = !GLU && NT <= 4;
+
 template <int TYPE, int NT, bool GLU, bool STAGED>
 __global__ void __launch_bounds__(kRowThreads, 2)
     gemm_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_up,
@@ -423,6 +428,8 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     const int in_window = TYPE == kQ6_K && STAGED ? at - min(at & ~15, (int)p.row_bytes - Cfg::RS) : 0;
     r0.fetch(row0 + stage, STAGED ? in_window : (off0 + at) & 15, t);
     r1.fetch(row1 + stage, STAGED ? in_window : (off1 + at) & 15, t);
+    float sum[NT][4] = {};  // of this superblock
+    float(&to)[NT][4] = kBySuperblock<NT, GLU> ? sum : acc;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
       uint32_t l0[4], h0[4], l1[4], h1[4];
@@ -432,11 +439,17 @@ __global__ void __launch_bounds__(kRowThreads, 2)
       for (int j = 0; j < NT; j++) {
         const uint4 xl = lds128(x_lane + stage + j * 8 * kTokenStride + 64 * w);
         const uint4 xh = lds128(x_lane + stage + j * 8 * kTokenStride + 64 * (4 + w));
-        mma_bf16(acc[j], l0[0], l1[0], l0[1], l1[1], xl.x, xl.y);
-        mma_bf16(acc[j], l0[2], l1[2], l0[3], l1[3], xl.z, xl.w);
-        mma_bf16(acc[j], h0[0], h1[0], h0[1], h1[1], xh.x, xh.y);
-        mma_bf16(acc[j], h0[2], h1[2], h0[3], h1[3], xh.z, xh.w);
+        mma_bf16(to[j], l0[0], l1[0], l0[1], l1[1], xl.x, xl.y);
+        mma_bf16(to[j], l0[2], l1[2], l0[3], l1[3], xl.z, xl.w);
+        mma_bf16(to[j], h0[0], h1[0], h0[1], h1[1], xh.x, xh.y);
+        mma_bf16(to[j], h0[2], h1[2], h0[3], h1[3], xh.z, xh.w);
       }
+    }
+    if constexpr (kBySuperblock<NT, GLU>) {
+#pragma unroll
+      for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[j][e] += sum[j][e];
     }
   }
   cp_async_wait<0>();
@@ -542,7 +555,7 @@ inline int rows_launch(RowsOnce &once, RowsKernel kernel, RowsParams &p, const C
     const long long clusters = (long long)blocks * tiles, rest = clusters % at_once * n;  // CTAs of the last wave
     const double load = clusters / at_once * 2.0 + (rest == 0 ? 0.0 : rest <= sms ? 1.3 : 2.0);
     double cost = load * (per + 0.75) + (n > 1 ? 0.5 : 0.0);
-    if (!p.epi.y_bf16 && 256 * per > kMaxF32Part) cost += 1e7 * per;  // the shortest parts if none is short enough
+    if (!p.epi.y_bf16 && tokens > 32 && 256 * per > kMaxF32Part) cost += 1e7 * per;  // the shortest parts if none is short enough
     if (cost < best) { best = cost; parts = n; }
   }
   p.per = (p.nsb + parts - 1) / parts;
