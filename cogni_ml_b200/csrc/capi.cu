@@ -100,8 +100,8 @@ int check_rows_call(const cogni_qmm_gemm_args *a, bool glu, RowsCall &c) {
   e.residual_bf16 = a->residual_type == COGNI_QMM_OUT_BF16;
   e.y = a->y; e.y_stride = a->y_stride; e.y_bf16 = a->y_type == COGNI_QMM_OUT_BF16;
   e.activation = a->activation;
-  e.vec = rows_vec4(e.y, e.y_stride, e.y_bf16) &&
-          (!e.residual || rows_vec4(e.residual, e.residual_stride, e.residual_bf16));
+  e.vec = rows_vec4(e.y, e.y_stride, e.y_bf16, a->n_out) &&
+          (!e.residual || rows_vec4(e.residual, e.residual_stride, e.residual_bf16, a->n_out));
   return COGNI_QMM_OK;
 }
 

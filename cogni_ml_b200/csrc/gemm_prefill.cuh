@@ -709,42 +709,43 @@ __device__ __forceinline__ void store_columns(const GemmParams &p, uint32_t tadd
 // holding one output each, as store_columns has it, took 20 us a tile for the residual's loads alone (Q4_K
 // 12288 x 4096, 4096 tokens, f32 residual: 471 us, bf16 552; without one 394).
 //
-// finish_columns: the columns of one round (part: [column][128] f32) from token `first` on, by the CTA's warps.  A function
-// of its own: inlined into the loop over the rounds, the constants of all activations stay in registers across it (80 more).
-__device__ __noinline__ void finish_columns(const RowEpilogue e, const float *part, int first, int live, int n, int n_out) {
+// finish_columns: the columns of one round (part: [column][128] f32) from token `first` on, by the CTA's warps.  The choice
+// of the activation encloses the rounds: inside them the constants of all activations would stay in registers (80 more).
+// Not a function of its own: as one, called with the epilogue's fields by value, it read a residual through the bias's pointer
+// in lanes that went element by element while others of their warp did not (n_out 11, rows of twelve).
+template <int ACT>
+__device__ __forceinline__ void finish_columns(const RowEpilogue &e, const float *part, int first, int live, int n, int n_out) {
   constexpr int kAhead = 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = (int)blockDim.x >> 5;
-  if (e.vec && n + 4 <= n_out) {
+  if (e.vec) {
+    if (n >= n_out) return;
     float bias[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) bias[i] = e.bias ? __ldg(e.bias + n + i) : 0.f;
-    with_activation(e.activation, [&](auto act) {
+    load_bias4(e.bias, n, n_out, bias);
 #pragma unroll 1
-      for (int c = warp; c < live; c += kAhead * nw) {
-        // the residual may be y itself: the loads of four tokens before the first store, so that they overlap
-        uint4 r[kAhead];
+    for (int c = warp; c < live; c += kAhead * nw) {
+      // the residual may be y itself: the loads of four tokens before the first store, so that they overlap
+      uint4 r[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; u++)
-          if (c + u * nw < live) r[u] = residual4_bits(e, first + c + u * nw, n);
+      for (int u = 0; u < kAhead; u++)
+        if (c + u * nw < live) r[u] = residual4_bits(e, first + c + u * nw, n);
 #pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-          if (c + u * nw >= live) break;
-          const float4 s = *reinterpret_cast<const float4 *>(part + (c + u * nw) * kBM + 4 * lane);
-          const float v[4] = {s.x, s.y, s.z, s.w};
-          float f[4];
-          residual4_values(e, r[u], f);
+      for (int u = 0; u < kAhead; u++) {
+        if (c + u * nw >= live) break;
+        const float4 s = *reinterpret_cast<const float4 *>(part + (c + u * nw) * kBM + 4 * lane);
+        const float v[4] = {s.x, s.y, s.z, s.w};
+        float f[4];
+        residual4_values(e, r[u], f);
 #pragma unroll
-          for (int i = 0; i < 4; i++) f[i] += activate<decltype(act)::value>(v[i] + bias[i]);
-          store_out4(e, first + c + u * nw, n, f);
-        }
+        for (int i = 0; i < 4; i++) f[i] += activate<ACT>(v[i] + bias[i]);
+        store_out4(e, first + c + u * nw, n, f);
       }
-    });
-  } else if (n < n_out) {
+    }
+  } else {
 #pragma unroll 1
     for (int c = warp; c < live; c += nw) {
       const float4 s = *reinterpret_cast<const float4 *>(part + c * kBM + 4 * lane);
       const float v[4] = {s.x, s.y, s.z, s.w};
-      epilogue_store4(e, v, first + c, n, n_out);
+      epilogue_store4_as<ACT>(e, v, first + c, n, n_out);
     }
   }
 }
@@ -753,23 +754,25 @@ template <int BN, int kChunks>
 __device__ __forceinline__ void epilogue_tile(const GemmParams &p, float *part, uint32_t taddr, int chunk, int m0, int n0, int q, int lane) {
   constexpr int kRound = BN < 256 ? BN : 256, kCols = kRound / kChunks;
   const int end = min(BN, p.m_rows - m0);
+  with_activation(p.epi.activation, [&](auto act) {
 #pragma unroll 1
-  for (int r0 = 0; r0 < end; r0 += kRound) {
-    const int live = min(kRound, end - r0);
-    if (chunk >= 0) {
+    for (int r0 = 0; r0 < end; r0 += kRound) {
+      const int live = min(kRound, end - r0);
+      if (chunk >= 0) {
 #pragma unroll 1
-      for (int c0 = chunk * kCols; c0 < (chunk + 1) * kCols && c0 < live; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld32(taddr + r0 + c0, v);
-        tmem_ld_wait();
+        for (int c0 = chunk * kCols; c0 < (chunk + 1) * kCols && c0 < live; c0 += 32) {
+          uint32_t v[32];
+          tmem_ld32(taddr + r0 + c0, v);
+          tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; j++) part[(c0 + j) * kBM + 32 * q + lane] = __uint_as_float(v[j]);
+          for (int j = 0; j < 32; j++) part[(c0 + j) * kBM + 32 * q + lane] = __uint_as_float(v[j]);
+        }
       }
+      __syncthreads();
+      finish_columns<decltype(act)::value>(p.epi, part, m0 + r0, live, n0 + 4 * lane, p.n_out);
+      __syncthreads();  // the columns have been read
     }
-    __syncthreads();
-    finish_columns(p.epi, part, m0 + r0, live, n0 + 4 * lane, p.n_out);
-    __syncthreads();  // the columns have been read
-  }
+  });
 }
 
 // At which of a superblock's four k-steps the copying thread fetches the next superblock's window.  It runs up to `stages`
@@ -1120,6 +1123,7 @@ __global__ void __launch_bounds__(threads_for(TYPE, STAGED, BN, TWO), TWO ? 2 : 
         prefetch_residual(p, m0 + R::epilogue_chunk(warp) * (BN / kChunks), BN / kChunks, n0 + 32 * q, lane);
     }
     mbar_wait(smem_u32(&bars[kAccBar]), 0);
+    __syncwarp();  // the lanes left the wait (and the prefetch) one by one; the loads of TMEM are the warp's
     tc_fence_after();
   }
   if (p.splits == 1) {
@@ -1431,6 +1435,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     constexpr int kCols = kPairBN / 4;
     if constexpr (MODE == kEpilogue) prefetch_residual(p, m0 + R::epilogue_chunk(warp) * kCols, kCols, n0 + 32 * q, lane);
     mbar_wait(smem_u32(&bars[kAccBar]), 0);
+    __syncwarp();  // the lanes left the wait (and the prefetch) one by one; the loads of TMEM are the warp's
     tc_fence_after();
     if constexpr (MODE != kEpilogue)
       store_columns<MODE>(p, taddr, R::epilogue_chunk(warp) * kCols, kCols, m0, n0, q, lane);
@@ -1775,7 +1780,7 @@ int launch_typed(RowsCall c, cudaStream_t s) {
           part.epi.residual = c.epi.y;
           part.epi.residual_stride = c.epi.y_stride;
           part.epi.residual_bf16 = 0;
-          part.epi.vec = rows_vec4(c.epi.y, c.epi.y_stride, false);
+          part.epi.vec = rows_vec4(c.epi.y, c.epi.y_stride, false, c.n_out);
         }
         return COGNI_QMM_OK;
       }

@@ -19,7 +19,7 @@ struct RowEpilogue {
   long long residual_stride, y_stride;  // elements between rows
   int residual_bf16, y_bf16;
   int activation;
-  int vec;  // four consecutive outputs from a multiple of four on are aligned for one access each
+  int vec;  // rows are multiples of four outputs, and four from a multiple of four on are aligned for one access each
 };
 
 template <int V> struct IntConst { static constexpr int value = V; };
@@ -56,13 +56,6 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// Plain loads, not through the read-only path: the residual may be the y that other threads write.
-__device__ __forceinline__ float load_residual(const RowEpilogue &e, int m, int n) {
-  if (!e.residual) return 0.f;
-  const long long at = (long long)m * e.residual_stride + n;
-  if (e.residual_bf16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(e.residual)[at]);
-  return reinterpret_cast<const float *>(e.residual)[at];
-}
 __device__ __forceinline__ void store_out(const RowEpilogue &e, int m, int n, float v) {
   const long long at = (long long)m * e.y_stride + n;
   if (e.y_bf16) reinterpret_cast<__nv_bfloat16 *>(e.y)[at] = __float2bfloat16_rn(v);
@@ -93,55 +86,65 @@ __device__ __forceinline__ void residual4_values(const RowEpilogue &e, const uin
   r[2] = e.residual_bf16 ? bf16_value(b.y) : __uint_as_float(b.z);
   r[3] = __uint_as_float(e.residual_bf16 ? b.y & 0xffff0000u : b.w);
 }
-// Four outputs n .. n + 3 (n a multiple of four) of row m, those below n_out.
-__device__ __forceinline__ void epilogue_store4(const RowEpilogue &e, const float (&sum)[4], int m, int n, int n_out) {
-  if (n >= n_out) return;
-  const bool vec = e.vec && n + 4 <= n_out;
-  float r[4], f[4];
-  if (vec) {
+// Residual and bias of four outputs n .. n + 3 (n a multiple of four below n_out) of row m.  Which accesses are taken is the same
+// for all lanes: outputs behind the row's end read its last element, and are not stored.  (Plain loads, not through the
+// read-only path: the residual may be the y that other threads write.)
+__device__ __forceinline__ void load_residual4(const RowEpilogue &e, int m, int n, int n_out, float (&r)[4]) {
+  if (e.vec || !e.residual) {
     residual4_values(e, residual4_bits(e, m, n), r);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = n + i < n_out ? load_residual(e, m, n + i) : 0.f;
+    return;
   }
+  const long long row = (long long)m * e.residual_stride;
 #pragma unroll
-  for (int i = 0; i < 4; i++) f[i] = sum[i] + (e.bias && n + i < n_out ? __ldg(e.bias + n + i) : 0.f);
-  with_activation(e.activation, [&](auto act) {
+  for (int i = 0; i < 4; i++) {
+    const long long at = row + min(n + i, n_out - 1);
+    r[i] = e.residual_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(e.residual)[at])
+                           : reinterpret_cast<const float *>(e.residual)[at];
+  }
+}
+__device__ __forceinline__ void load_bias4(const float *bias, int n, int n_out, float (&b)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = r[i] + activate<decltype(act)::value>(f[i]);
-  });
-  if (vec) {
+  for (int i = 0; i < 4; i++) b[i] = bias ? __ldg(bias + min(n + i, n_out - 1)) : 0.f;
+}
+__device__ __forceinline__ void store_outputs4(const RowEpilogue &e, int m, int n, int n_out, const float (&f)[4]) {
+  if (e.vec) {
     store_out4(e, m, n, f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (n + i < n_out) store_out(e, m, n + i, f[i]);
+    return;
   }
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (n + i < n_out) store_out(e, m, n + i, f[i]);
+}
+// Four outputs n .. n + 3 (n a multiple of four) of row m, those below n_out.
+template <int ACT> __device__ __forceinline__ void epilogue_store4_as(const RowEpilogue &e, const float (&sum)[4], int m, int n, int n_out) {
+  if (n >= n_out) return;
+  float r[4], b[4], f[4];
+  load_residual4(e, m, n, n_out, r);
+  load_bias4(e.bias, n, n_out, b);
+#pragma unroll
+  for (int i = 0; i < 4; i++) f[i] = r[i] + activate<ACT>(sum[i] + b[i]);
+  store_outputs4(e, m, n, n_out, f);
+}
+__device__ __forceinline__ void epilogue_store4(const RowEpilogue &e, const float (&sum)[4], int m, int n, int n_out) {
+  with_activation(e.activation, [&](auto act) { epilogue_store4_as<decltype(act)::value>(e, sum, m, n, n_out); });
 }
 __device__ __forceinline__ void glu_store4(const RowEpilogue &e, const float (&gate)[4], const float (&up)[4], int m,
                                            int n, int n_out) {
   if (n >= n_out) return;
-  float f[4];
+  float bg[4], bu[4], f[4];
+  load_bias4(e.bias, n, n_out, bg);
+  load_bias4(e.bias_up, n, n_out, bu);
   with_activation(e.activation, [&](auto act) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const bool in = n + i < n_out;
-      f[i] = activate<decltype(act)::value>(gate[i] + (e.bias && in ? __ldg(e.bias + n + i) : 0.f)) *
-             (up[i] + (e.bias_up && in ? __ldg(e.bias_up + n + i) : 0.f));
-    }
+    for (int i = 0; i < 4; i++) f[i] = activate<decltype(act)::value>(gate[i] + bg[i]) * (up[i] + bu[i]);
   });
-  if (e.vec && n + 4 <= n_out) {
-    store_out4(e, m, n, f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (n + i < n_out) store_out(e, m, n + i, f[i]);
-  }
+  store_outputs4(e, m, n, n_out, f);
 }
 
-// Whether four consecutive elements of every row can be one access (rows `stride` elements apart).
-inline bool rows_vec4(const void *p, long long stride, bool bf16) {
-  return (reinterpret_cast<uintptr_t>(p) & (bf16 ? 7 : 15)) == 0 && stride % 4 == 0;
+// Whether four consecutive elements of every row of n can be one access (rows `stride` elements apart), the last ones too: a
+// row that ends inside four outputs goes element by element in all lanes.
+inline bool rows_vec4(const void *p, long long stride, bool bf16, int n) {
+  return (reinterpret_cast<uintptr_t>(p) & (bf16 ? 7 : 15)) == 0 && stride % 4 == 0 && n % 4 == 0;
 }
 
 // One call of a product with an epilogue, as the launchers take it.
