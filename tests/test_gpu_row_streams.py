@@ -80,3 +80,26 @@ def test_norm_vectors_and_biases_live_until_they_are_read(cuda, oracle, engine):
     torch.cuda.synchronize()
     assert torch.equal(y, want[0]) and torch.equal(z, want[1])
     del over
+
+
+def test_side_streams_in_a_captured_graph(cuda, oracle, engine):
+    """Two calls on two streams between a fork and a join, captured once and replayed on new inputs."""
+    x, ops = setup(cuda, oracle)
+    for op in OPS:
+        ops[op](x, None)
+    torch.cuda.synchronize()
+    sides = torch.cuda.Stream(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        current = torch.cuda.current_stream()
+        for s in sides:
+            s.wait_stream(current)
+        got = [ops[op](x, s) for op, s in (("glu", sides[0]), ("epilogue", sides[1]), ("norm", sides[0]), ("hidden", sides[1]))]
+        for s in sides:
+            current.wait_stream(s)
+    for seed in (5, 6):
+        x.copy_(rows(cuda, x.shape[0], x.shape[1], seed, torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        for op, y in zip(("glu", "epilogue", "norm", "hidden"), got):
+            assert torch.equal(y, ops[op](x, None)), op
