@@ -1748,9 +1748,9 @@ int launch_plan(const RowsCall &c, const TilePlan &plan, cudaStream_t s) {
   return launch<TYPE, 128, false, MODE>(c, splits, s);
 }
 
-// What a launch after another costs beside its tiles, us: its start, and y read once more; where the times below lie, Q4_K
-// and Q5_K take clusters and the other types turns.
-constexpr double kTurnCost = 7.0;
+// What a launch after another costs beside its tiles, us: its start, and y read once more.  (At 1.0 turns are taken where they
+// were the faster ones, on 1024 to 4096 rows x 4096 x 8192 and 12288 of five types; at 7.0 Q4_K and Q5_K took clusters.)
+constexpr double kTurnCost = 1.0;
 
 template <int TYPE, int MODE>
 int launch_typed(RowsCall c, cudaStream_t s) {
@@ -1761,8 +1761,8 @@ int launch_typed(RowsCall c, cudaStream_t s) {
   if constexpr (MODE == kEpilogue) {
     // An f32 y whose parts of K have a limit (kMaxF32Part), where no activation follows the sum: the parts may also be
     // launches one after the other, each adding to what the one before left in y.  That spares the exchange of a cluster and
-    // the tiles that it leaves without a partner.  4096 x 12288, 2048 rows, f32 residual, us, clusters / turns (K whole):
-    // Q4_K 190 / 195 (172), Q6_K 222 / 197 (174), Q8_0 258 / 226 (203), IQ4_NL 213 / 188 (168).
+    // the tiles that it leaves without a partner.  4096 x 12288, 2048 rows, f32 residual, us, clusters / turns: Q4_K 188 / 176,
+    // Q6_K 223 / 195, Q8_0 260 / 223, IQ4_NL 215 / 188 (one launch over all of K: 172, 174, 203, 168).
     const int turns = (nks * kBK + kMaxF32Part - 1) / kMaxF32Part;
     if (turns > 1 && !c.epi.y_bf16 && c.epi.activation == COGNI_QMM_ACT_NONE && g_prefill_force_split == 0) {
       const int per = ksteps_per_split(nks, turns);
