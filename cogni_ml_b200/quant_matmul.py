@@ -323,7 +323,8 @@ class DeviceQuantWeight:
         activation: one of ACTIVATIONS.  bias f32 [out_dim]; residual [M, out_dim] f32 or bf16, which may
         be `out` itself (other overlaps of out and an input are refused).  Rows of x, residual and out may be strided (x by a multiple of eight
         elements).  A weight enters as bf16(dequant(W)), as in `gemm`.  With `stream` the caller orders the inputs before
-        the call there and the result's readers after it; their memory is kept until that stream is done with it."""
+        the call there and the result's readers after it; their memory is kept until that stream is done with it.
+        (A single f32 row, with or without a residual, is `gemv`'s in less time.)"""
         return _gemm_rows(self, None, x, bias, None, activation, residual, out_dtype, out, stream)
 
 
