@@ -544,7 +544,10 @@ inline int rows_launch(RowsOnce &once, RowsKernel kernel, RowsParams &p, const C
                        int sms, cudaStream_t s) {
   const int blocks = (p.n_out + outs - 1) / outs, tiles = (p.m_rows + tokens - 1) / tokens;
   // Parts of K.  Clusters of n CTAs come in waves of as many as fit the GPU, two CTAs an SM; a CTA takes its superblocks
-  // and a start and an end, beside another one not twice as long as alone.
+  // and a start and an end, beside another one not twice as long as alone.  Measured over every split, both forms, five types, 1 to
+  // 48 tokens: with these constants 1.1 % over the best on average for 1024 to 17408 rows of 4096 to 17408 columns as layers have
+  // them, 2.6 % for drawn shapes (126 of 1122 more than 10 %).  1.75 instead of 1.3 and 1.0 instead of 0.75 make that 0.9 %, but
+  // 12288 x 4096 onto f32 takes 9 to 25 % longer with them.
   int parts = 1;
   double best = 1e30;
   for (int n = 1; n <= 8 && n <= p.nsb; n++) {
